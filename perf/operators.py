@@ -23,29 +23,29 @@ E4M3_MAX = 448.0
 def listed():
     return [
         # one request's token ahead of an e4m3 feed-forward layer of width 512: latency
-        {"name": "norm quant, one row", "op": "norm_quant", "rows": 1, "cols": 512, "type": "bf16"},
+        {"name": "norm quant one row", "op": "norm_quant", "rows": 1, "cols": 512, "type": "bf16"},
         # all tokens of a training or scoring batch at the model's width
-        {"name": "norm quant, 262144 x 512", "op": "norm_quant", "rows": 262144, "cols": 512, "type": "bf16"},
+        {"name": "norm quant 262144 x 512", "op": "norm_quant", "rows": 262144, "cols": 512, "type": "bf16"},
         # a wide tokenizer's rows (2560 = 20 fields of 128), a batch whose rows fill no tile
-        {"name": "norm quant, 5003 x 2560", "op": "norm_quant", "rows": 5003, "cols": 2560, "type": "fp16"},
+        {"name": "norm quant 5003 x 2560", "op": "norm_quant", "rows": 5003, "cols": 2560, "type": "fp16"},
         # the training step's backward pass at the model's width
-        {"name": "norm backward, 65536 x 512", "op": "norm_backward", "rows": 65536, "cols": 512, "type": "bf16"},
+        {"name": "norm backward 65536 x 512", "op": "norm_backward", "rows": 65536, "cols": 512, "type": "bf16"},
         # parity training in full precision on wide rows, few of them
-        {"name": "norm backward, 1201 x 4096", "op": "norm_backward", "rows": 1201, "cols": 4096, "type": "fp32"},
+        {"name": "norm backward 1201 x 4096", "op": "norm_backward", "rows": 1201, "cols": 4096, "type": "fp32"},
         # gated layer of 512 -> 2 x 2048: the activation of a training batch and what it keeps
-        {"name": "gate, 32768 x 2048", "op": "gate", "rows": 32768, "hidden": 2048, "gated": True, "type": "bf16"},
+        {"name": "gate 32768 x 2048", "op": "gate", "rows": 32768, "hidden": 2048, "gated": True, "type": "bf16"},
         # its backward pass from the kept 8 bits
-        {"name": "gate backward, 32768 x 2048", "op": "gate_backward", "rows": 32768, "hidden": 2048, "gated": True, "type": "bf16"},
+        {"name": "gate backward 32768 x 2048", "op": "gate_backward", "rows": 32768, "hidden": 2048, "gated": True, "type": "bf16"},
         # a small ungated layer, ragged rows
-        {"name": "gate backward, 777 x 640", "op": "gate_backward", "rows": 777, "hidden": 640, "gated": False, "type": "fp16"},
+        {"name": "gate backward 777 x 640", "op": "gate_backward", "rows": 777, "hidden": 640, "gated": False, "type": "fp16"},
         # a few requests' tokens routed over sixteen experts: the weights are the traffic
-        {"name": "experts, 24 rows", "op": "experts", "rows": 24, "experts": 16, "k": 512, "n": 2048, "silu": True, "type": "bf16"},
+        {"name": "experts 24 rows", "op": "experts", "rows": 24, "experts": 16, "k": 512, "n": 2048, "silu": True, "type": "bf16"},
         # a training batch through the up projections of nine parameter groups
-        {"name": "experts, 65536 rows", "op": "experts", "rows": 65536, "experts": 9, "k": 512, "n": 2048, "silu": False, "type": "bf16"},
+        {"name": "experts 65536 rows", "op": "experts", "rows": 65536, "experts": 9, "k": 512, "n": 2048, "silu": False, "type": "bf16"},
         # gradients of rows, weights and biases of such a layer
-        {"name": "experts backward, 32768 rows", "op": "experts_backward", "rows": 32768, "experts": 16, "k": 512, "n": 2048, "type": "bf16"},
+        {"name": "experts backward 32768 rows", "op": "experts_backward", "rows": 32768, "experts": 16, "k": 512, "n": 2048, "type": "bf16"},
         # odd widths and ragged groups, some of them empty
-        {"name": "experts backward, 1999 rows", "op": "experts_backward", "rows": 1999, "experts": 12, "k": 520, "n": 1000, "type": "fp16"},
+        {"name": "experts backward 1999 rows", "op": "experts_backward", "rows": 1999, "experts": 12, "k": 520, "n": 1000, "type": "fp16"},
     ]
 
 
