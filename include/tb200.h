@@ -130,6 +130,39 @@ int tb200_rmsnorm_bwd(const void* x, const void* gamma, const void* dy, void* dx
 int tb200_layernorm_bwd(const void* x, const void* gamma, const void* dy, void* dx, void* dgamma, void* dbeta,
                         float* workspace, int64_t rows, int32_t cols, float eps, int dtype, void* stream);
 
+/* Residual addition and RMSNorm in one pass (the pre-norm of a block: `x = x + attention(...)`, `ffn_norm(x)`,
+ * experiments/onetrans/model.py:106-107), with the result in the tensors' type, in e4m3 with scales, or both:
+ *     t = x + residual;  total = t;  normed = t * rsqrt(mean(t^2) + eps) * gamma;  q = e4m3(normed / scale)
+ * residual may be NULL (t = x).  total, normed and q may each be NULL, not all of them.  The statistics and the 8-bit
+ * values come from t and normed in fp32, before they are rounded.  scale_kind: 0 = no q; 1 = fp32 [rows, cols / 128],
+ * amax / 448 of each 1 x 128 block (the operand of tb200_fp8_gemm); 2 = power-of-two scale atoms (the operand of
+ * tb200_mx_gemm; the caller zeroes the atoms of rows behind the last).  cols: a multiple of 8 up to 16384, of 128 where q
+ * is written.  No output may overlap an input. */
+int tb200_add_rmsnorm_fwd(const void* x, const void* residual, const void* gamma, void* total, void* normed, void* q,
+                          void* scales, int32_t scale_kind, int64_t rows, int32_t cols, float eps, int dtype, void* stream);
+/* Its gradients from `total` and the upstream gradients of normed and of total (d_total may be NULL): d_in is the gradient
+ * of x and of residual alike, dgamma that of gamma; the statistics are recomputed from total.  workspace: device floats of
+ * tb200_add_rmsnorm_bwd_workspace_bytes(cols) bytes, for this call alone.  The sums run in a fixed order. */
+int64_t tb200_add_rmsnorm_bwd_workspace_bytes(int32_t cols);
+int tb200_add_rmsnorm_bwd(const void* total, const void* gamma, const void* d_normed, const void* d_total, void* d_in,
+                          void* dgamma, float* workspace, int64_t rows, int32_t cols, float eps, int dtype, void* stream);
+
+/* Activations kept in 8 bits for the backward pass: q e4m3 [rows, cols], scales fp32 [rows, cols / 128] = the smallest
+ * power of two s with max|x| / s <= 448 over the finite values of the block; values that are not finite are kept as NaN.
+ * x / s and q s are exact.  cols % 128 == 0. */
+int tb200_keep_fwd(const void* x, void* q, float* scales, int64_t rows, int32_t cols, int dtype, void* stream);
+int tb200_keep_restore(const void* q, const float* scales, void* x, int64_t rows, int32_t cols, int dtype, void* stream);
+/* The activation of a feed-forward layer: h [rows, hidden] = silu(gate) * value of up [rows, 2 hidden] = [gate | value]
+ * (gate_first, experiments/tokenformer/model.py:118-128) or [value | gate] (experiments/baseline/model.py:99-113), or
+ * silu(up) of up [rows, hidden] (gated = 0, experiments/onetrans/model.py:33-44).  q, scales (both or neither): `up` kept
+ * as above.  hidden % 128 == 0. */
+int tb200_silu_gate_fwd(const void* up, void* h, void* q, float* scales, int64_t rows, int32_t hidden, int32_t gated,
+                        int32_t gate_first, int dtype, void* stream);
+/* Its gradient dup from the kept values and dh; h (may be NULL) receives the activation again, for the weight gradient of
+ * the layer behind it.  dtype: of dh, dup and h. */
+int tb200_silu_gate_bwd(const void* q, const float* scales, const void* dh, void* dup, void* h, int64_t rows, int32_t hidden,
+                        int32_t gated, int32_t gate_first, int dtype, void* stream);
+
 /* The whole sequence tokenizer in one kernel: row gather -> projection -> SiLU -> LayerNorm -> time / position rows
  * -> first RMSNorm,
  *     x[r, :]      = concat_f tables[f][clamp(ids[f, r]), :]                     (K = n_feat * emb columns)

@@ -22,10 +22,9 @@
 // way, fetched by TMA while the K loop runs.
 // Every wait on an mbarrier is bounded; a wait that gives up raises the status word and all roles
 // drain out through the same final barrier, where the TMEM allocation is released.
-#include <cuda_fp8.h>
-
 #include <mutex>
 
+#include "quant.cuh"
 #include "tb200_common.cuh"
 #include "tb200_ptx.cuh"
 #include "tb200_tmap.cuh"
@@ -74,13 +73,6 @@ __device__ __forceinline__ float silu(float x) {
     float t;
     asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(h));
     return fmaf(h, t, h);
-}
-
-// 64 fp32 -> 64 e4m3 bytes (as 16 words) with q = x * inv_scale, round-to-nearest, saturating
-__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
-    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 
 // Work distribution: a CTA keeps ONE column tile (256 weight rows) for its whole life and walks down

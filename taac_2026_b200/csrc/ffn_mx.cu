@@ -29,8 +29,7 @@
 // the same final barrier, where the TMEM allocation is released.
 #include <cstdlib>
 
-#include <cuda_fp8.h>
-
+#include "quant.cuh"
 #include "tb200_common.cuh"
 #include "tb200_ptx.cuh"
 #include "tb200_tmap.cuh"
@@ -47,7 +46,6 @@ constexpr int kThreads = 576;
 constexpr int kEpiThreads = 512;
 constexpr uint32_t kABytes = kBM * kBK;      // 16 KB
 constexpr uint32_t kBBytes = kBN * kBK;      // 32 KB
-constexpr uint32_t kSfAtom = 512;            // scale factors of 128 rows x one K block
 constexpr uint32_t kSfaBytes = kSfAtom;      // A: 128 rows
 constexpr uint32_t kSfbBytes = 2 * kSfAtom;  // B: 256 rows
 constexpr uint32_t kTmemCols = 512;          // accumulator 256 + two scale-factor slots of 12 columns (allocation: power of two)
@@ -80,27 +78,6 @@ __device__ __forceinline__ float silu(float x) {
     asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(h));
     return fmaf(h, t, h);
 }
-
-// Smallest power of two s with amax / s <= 448, as its UE8M0 byte (s = 2^(byte - 127)), and 1 / s.
-__device__ __forceinline__ uint32_t pow2_scale(float amax, float* inv) {
-    int e = 0;
-    if (amax > 0.f) {
-        const uint32_t bits = __float_as_uint(amax * (1.0f / 448.0f));
-        e = static_cast<int>((bits >> 23) & 0xFF) - 127 + ((bits & 0x7FFFFFu) != 0u ? 1 : 0);
-        e = max(-126, min(e, 126));
-    }
-    *inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    return static_cast<uint32_t>(e + 127);
-}
-
-__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
-    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
-}
-
-// byte offset of row r's four slice bytes inside a scale atom
-__host__ __device__ __forceinline__ uint32_t sf_row_offset(int r) { return static_cast<uint32_t>((r & 31) * 16 + (r >> 5) * 4); }
 
 // Work distribution as in the amax/448 kernel: a CTA keeps ONE column tile for its whole life and walks down the row
 // tiles; the CTAs that share a row tile read it at about the same time, so activations come from HBM once.

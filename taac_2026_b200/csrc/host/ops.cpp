@@ -533,6 +533,140 @@ PyObject* py_ffn_mx(PyObject*, PyObject* const* args, Py_ssize_t) {
     END_HANDLE_TH_ERRORS
 }
 
+// -------------------------------------------------------------------------------------------- residual addition + norm, kept activations
+bool on16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+// a dense operand of this type on the other's device, on a 16-byte boundary
+bool plain(const Tensor& t, at::ScalarType type, const Tensor& beside) {
+    return dense(t, type) && t.device() == beside.device() && on16(t);
+}
+template <typename... Ts>
+PyObject* tuple_of(const Ts&... t) {
+    PyObject* items[] = {(t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None))...};
+    PyObject* out = PyTuple_New(sizeof...(Ts));
+    for (size_t i = 0; i < sizeof...(Ts); ++i) PyTuple_SET_ITEM(out, i, items[i]);
+    return out;
+}
+std::vector<int64_t> sizes_with(const Tensor& t, int64_t last) {
+    auto s = t.sizes().vec();
+    s.back() = last;
+    return s;
+}
+
+// add_rms_norm(x, residual or None, weight, eps, kind): kind 0 -> (total, normed), 1 / 2 -> (total, q, scales)
+PyObject* py_add_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    if (!is_tensor(args[0]) || !is_optional(args[1]) || !is_tensor(args[2])) Py_RETURN_NONE;
+    const Tensor& x = tensor(args[0]);
+    const auto residual = optional_tensor(args[1]);
+    const Tensor& w = tensor(args[2]);
+    const double eps = number(args[3]);
+    const int64_t kind = integer(args[4]);
+    const auto t = x.scalar_type();
+    if (x.dim() < 2 || w.dim() != 1 || x.size(-1) != w.size(0) || dtype_code(t) < 0 || !plain(x, t, x) || !plain(w, t, x) || x.numel() == 0 ||
+        x.size(-1) > INT32_MAX)
+        Py_RETURN_NONE;
+    if (residual.has_value() ? (!plain(*residual, t, x) || residual->sizes() != x.sizes()) : kind == 0) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(x.device());
+    if (!tb200_device_ok()) Py_RETURN_NONE;
+    const int64_t cols = x.size(-1), rows = x.numel() / cols;
+    const auto opt = x.options().requires_grad(false);
+    Tensor total, normed, q, scales;
+    if (residual.has_value()) total = at::empty(x.sizes(), opt);
+    if (kind == 0) {
+        normed = at::empty(x.sizes(), opt);
+    } else {
+        q = at::empty(x.sizes(), opt.dtype(at::kFloat8_e4m3fn));
+        const std::vector<int64_t> atoms{(rows + 127) / 128, cols / 128, 512};
+        if (kind == 1) scales = at::empty(sizes_with(x, cols / 128), opt.dtype(at::kFloat));
+        else scales = rows % 128 == 0 ? at::empty(atoms, opt.dtype(at::kByte)) : at::zeros(atoms, opt.dtype(at::kByte));
+    }
+    auto at_of = [](const Tensor& v) -> void* { return v.defined() ? v.data_ptr() : nullptr; };
+    if (tb200_add_rmsnorm_fwd(ptr(x), ptr(residual), ptr(w), at_of(total), at_of(normed), at_of(q), at_of(scales), static_cast<int32_t>(kind), rows,
+                              static_cast<int32_t>(cols), static_cast<float>(eps), dtype_code(t), stream_of(x)) != TB200_OK)
+        Py_RETURN_NONE;
+    if (!residual.has_value()) total = x;
+    return kind == 0 ? tuple_of(total, normed) : tuple_of(total, q, scales);
+    END_HANDLE_TH_ERRORS
+}
+
+// add_rms_norm_backward(total, weight, grad_normed, grad_total or None, eps) -> (grad, dweight)
+PyObject* py_add_rms_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    if (!is_tensor(args[0]) || !is_tensor(args[1]) || !is_tensor(args[2]) || !is_optional(args[3])) Py_RETURN_NONE;
+    const Tensor& total = tensor(args[0]);
+    const Tensor& w = tensor(args[1]);
+    const Tensor& dn = tensor(args[2]);
+    const auto dt = optional_tensor(args[3]);
+    const double eps = number(args[4]);
+    const auto t = total.scalar_type();
+    if (total.dim() < 2 || w.dim() != 1 || total.size(-1) != w.size(0) || dtype_code(t) < 0 || !plain(total, t, total) || !plain(w, t, total) ||
+        !plain(dn, t, total) || dn.sizes() != total.sizes() || total.numel() == 0 || total.size(-1) > INT32_MAX)
+        Py_RETURN_NONE;
+    if (dt.has_value() && (!plain(*dt, t, total) || dt->sizes() != total.sizes())) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(total.device());
+    if (!tb200_device_ok()) Py_RETURN_NONE;
+    const int64_t cols = total.size(-1), rows = total.numel() / cols;
+    const auto opt = total.options().requires_grad(false);
+    Tensor grad = at::empty(total.sizes(), opt), dw = at::empty(w.sizes(), opt);
+    Tensor work = at::empty({tb200_add_rmsnorm_bwd_workspace_bytes(static_cast<int32_t>(cols)) / 4}, opt.dtype(at::kFloat));
+    if (tb200_add_rmsnorm_bwd(ptr(total), ptr(w), ptr(dn), ptr(dt), ptr(grad), ptr(dw), static_cast<float*>(ptr(work)), rows,
+                              static_cast<int32_t>(cols), static_cast<float>(eps), dtype_code(t), stream_of(total)) != TB200_OK)
+        Py_RETURN_NONE;
+    return tuple_of(grad, dw);
+    END_HANDLE_TH_ERRORS
+}
+
+// silu_gate(up, gated, gate_first, keep) -> h or (h, q, scales)
+PyObject* py_silu_gate(PyObject*, PyObject* const* args, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    if (!is_tensor(args[0])) Py_RETURN_NONE;
+    const Tensor& up = tensor(args[0]);
+    const bool gated = truth(args[1]), first = truth(args[2]), keep = truth(args[3]);
+    const auto t = up.scalar_type();
+    if (up.dim() < 1 || dtype_code(t) < 0 || !plain(up, t, up) || up.numel() == 0 || up.size(-1) % (gated ? 256 : 128) != 0 || up.size(-1) > INT32_MAX)
+        Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(up.device());
+    if (!tb200_device_ok()) Py_RETURN_NONE;
+    const int64_t width = up.size(-1), hidden = gated ? width / 2 : width, rows = up.numel() / width;
+    const auto opt = up.options().requires_grad(false);
+    Tensor h = at::empty(sizes_with(up, hidden), opt), q, scales;
+    if (keep) {
+        q = at::empty(up.sizes(), opt.dtype(at::kFloat8_e4m3fn));
+        scales = at::empty(sizes_with(up, width / 128), opt.dtype(at::kFloat));
+    }
+    if (tb200_silu_gate_fwd(ptr(up), ptr(h), keep ? ptr(q) : nullptr, keep ? static_cast<float*>(ptr(scales)) : nullptr, rows,
+                            static_cast<int32_t>(hidden), gated, first, dtype_code(t), stream_of(up)) != TB200_OK)
+        Py_RETURN_NONE;
+    return keep ? tuple_of(h, q, scales) : THPVariable_Wrap(h);
+    END_HANDLE_TH_ERRORS
+}
+
+// silu_gate_backward(q, scales, grad, gated, gate_first, activation) -> (grad_up, h or None)
+PyObject* py_silu_gate_backward(PyObject*, PyObject* const* args, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    if (!is_tensor(args[0]) || !is_tensor(args[1]) || !is_tensor(args[2])) Py_RETURN_NONE;
+    const Tensor& q = tensor(args[0]);
+    const Tensor& scales = tensor(args[1]);
+    const Tensor& dh = tensor(args[2]);
+    const bool gated = truth(args[3]), first = truth(args[4]), activation = truth(args[5]);
+    const auto t = dh.scalar_type();
+    if (q.dim() < 1 || dtype_code(t) < 0 || !plain(q, at::kFloat8_e4m3fn, q) || !plain(dh, t, q) || !dense(scales, at::kFloat) ||
+        scales.device() != q.device() || q.numel() == 0 || q.size(-1) % (gated ? 256 : 128) != 0 || q.size(-1) > INT32_MAX)
+        Py_RETURN_NONE;
+    const int64_t width = q.size(-1), hidden = gated ? width / 2 : width, rows = q.numel() / width;
+    if (scales.sizes() != c10::IntArrayRef(sizes_with(q, width / 128)) || dh.sizes() != c10::IntArrayRef(sizes_with(q, hidden))) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(q.device());
+    if (!tb200_device_ok()) Py_RETURN_NONE;
+    const auto opt = dh.options().requires_grad(false);
+    Tensor dup = at::empty(q.sizes(), opt), h;
+    if (activation) h = at::empty(dh.sizes(), opt);
+    if (tb200_silu_gate_bwd(ptr(q), static_cast<float*>(ptr(scales)), ptr(dh), ptr(dup), activation ? ptr(h) : nullptr, rows,
+                            static_cast<int32_t>(hidden), gated, first, dtype_code(t), stream_of(q)) != TB200_OK)
+        Py_RETURN_NONE;
+    return tuple_of(dup, h);
+    END_HANDLE_TH_ERRORS
+}
+
 #define TB200_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     TB200_METHOD(rms_norm),
@@ -544,6 +678,10 @@ PyMethodDef methods[] = {
     TB200_METHOD(ffn_fp8),
     TB200_METHOD(ffn_fp8_precise),
     TB200_METHOD(ffn_mx),
+    TB200_METHOD(add_rms_norm),
+    TB200_METHOD(add_rms_norm_backward),
+    TB200_METHOD(silu_gate),
+    TB200_METHOD(silu_gate_backward),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Host side of the operator calls.", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -192,6 +192,48 @@ struct Vec16<__half> {
     }
 };
 
+// Eight consecutive values as they lie in memory: one 16-byte piece of a 16-bit type, two of fp32
+template <typename T>
+struct Octet {
+    static constexpr int P = sizeof(T) / 2;      // 16-byte pieces
+    uint4 v[P];
+    __device__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w)
+                         : "l"(p + i * (8 / P)));
+    }
+    __device__ void load_cached(const T* p) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ void clear() {
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ void unpack(float (&f)[8]) const {
+        constexpr int N = Vec16<T>::N;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float g[N];
+            Vec16<T>::unpack(v[i], g);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[i * N + e] = g[e];
+        }
+    }
+    static __device__ void store(T* p, const float (&f)[8]) {
+        constexpr int N = Vec16<T>::N;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float g[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) g[e] = f[i * N + e];
+            *(reinterpret_cast<uint4*>(p) + i) = Vec16<T>::pack(g);
+        }
+    }
+};
+
 template <typename T>
 __device__ __forceinline__ float to_float(T v);
 template <>

@@ -23,6 +23,7 @@ from dataclasses import dataclass
 from typing import Any, Literal, Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from taac_2026_b200 import _lib
 
@@ -57,9 +58,13 @@ def _require_cuda_tensors(operator_name: str, *tensors: torch.Tensor | None) -> 
     return checked[0].device
 
 
-def _require_backend(operator_name: str, backend: str) -> None:
+def _require_backend_name(operator_name: str, backend: str) -> None:
     if backend != "cuda":
         raise ValueError(f"unsupported {operator_name} backend: {backend}")
+
+
+def _require_backend(operator_name: str, backend: str) -> None:
+    _require_backend_name(operator_name, backend)
     if not cuda_available():
         raise RuntimeError("cuda backend requested but libtb200 or an sm_100 CUDA device is not available")
 
@@ -367,6 +372,152 @@ def layer_norm(
         )
     _lib.check(code, "cuda layer_norm")
     return out.reshape(original_shape)
+
+
+# --------------------------------------------------------------------------------------------
+# residual addition + RMSNorm, with an 8-bit result
+# --------------------------------------------------------------------------------------------
+_SCALE_KINDS = {"1x128": 1, "mx": 2}
+ADD_NORM_MAX_COLS = 16384
+
+
+def _normalize_add_rms_norm_inputs(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, name: str, width: int):
+    if x.ndim < 2:
+        raise ValueError(f"{name} expects input with at least 2 dimensions")
+    if weight.ndim != 1:
+        raise ValueError(f"{name} weight must be a 1D tensor")
+    if x.shape[-1] != weight.shape[0]:
+        raise ValueError(f"last dimension {x.shape[-1]} does not match weight size {weight.shape[0]}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"{name} residual must have the input's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if residual is not None and residual.dtype != x.dtype:
+        raise ValueError(f"{name} residual must have the input's dtype {x.dtype}, got {residual.dtype}")
+    if x.shape[-1] % width or not 0 < x.shape[-1] <= ADD_NORM_MAX_COLS:
+        raise ValueError(f"{name} needs the last dimension to be a multiple of {width} of at most {ADD_NORM_MAX_COLS}")
+    _require_backend(name, "cuda")
+    _require_cuda_tensors(f"cuda {name}", x, residual)
+    if x.dtype not in _DTYPE_CODES:
+        raise RuntimeError(f"cuda {name} does not support dtype {x.dtype}")
+    matrix = _aligned(x.reshape(-1, x.shape[-1]))
+    res = None if residual is None else _aligned(residual.reshape(matrix.shape))
+    return matrix, res, _aligned(weight.to(device=matrix.device, dtype=matrix.dtype))
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """`t` contiguous and on a 16-byte boundary (a view into the middle of a buffer may be on neither)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _add_rms_norm(x, residual, weight, eps, name, *, normed: bool, scales: str | None):
+    """(total or None, normed or None, q or None, scales or None) of one launch."""
+    matrix, res, w = _normalize_add_rms_norm_inputs(x, residual, weight, name, 8 if scales is None else 128)
+    rows, cols = matrix.shape
+    dev = matrix.device
+    total = None if res is None else torch.empty_like(matrix)
+    out = torch.empty_like(matrix) if normed else None
+    q = sc = None
+    if scales is not None:
+        q = torch.empty(matrix.shape, dtype=torch.float8_e4m3fn, device=dev)
+        if scales == "mx":      # the atoms of a ragged last tile hold zeros for the rows behind the end
+            make = torch.empty if rows % 128 == 0 else torch.zeros
+            sc = make((rows + 127) // 128, cols // 128, 512, dtype=torch.uint8, device=dev)
+        else:
+            sc = torch.empty(rows, cols // 128, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev), _timed("add_rms_norm", rows=rows, cols=cols, esize=matrix.element_size(), quant=scales or ""):
+        code = _lib.load().tb200_add_rmsnorm_fwd(_ptr(matrix), _ptr(res), _ptr(w), _ptr(total), _ptr(out), _ptr(q), _ptr(sc),
+                                                 _SCALE_KINDS.get(scales, 0), rows, cols, float(eps), _DTYPE_CODES[matrix.dtype], _stream_ptr())
+    _lib.check(code, f"cuda {name}")
+    shape = x.shape
+    return (x if total is None else total.view(shape), None if out is None else out.view(shape), None if q is None else q.view(shape),
+            sc if sc is None or scales == "mx" else sc.view(*shape[:-1], cols // 128))
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, backend: str = "cuda"
+                 ) -> tuple[torch.Tensor, torch.Tensor]:
+    """``total = x + residual`` and ``normed = rms_norm(total, weight, eps)`` in one pass: the residual stream and the input
+    of a block's next layer (`x + attention(...)`, `ffn_norm`: experiments/onetrans/model.py:106-107).
+
+    The statistics come from the sum in fp32, before it is rounded.  Differentiable: both results may have upstream
+    gradients.  The width is a multiple of 8, at most 16384."""
+    _require_backend_name("add_rms_norm", backend)
+    if residual is None:
+        raise ValueError("add_rms_norm needs a residual; rms_norm serves a single input")
+    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or weight.requires_grad):
+        _normalize_add_rms_norm_inputs(x, residual, weight, "add_rms_norm", 8)
+        return _AddRmsNormFunction.apply(x, residual, weight, float(eps))
+    if _TIMING is None:
+        fast = _host.add_rms_norm(x, residual, weight, eps, 0)
+        if fast is not None:
+            return fast
+    total, normed, _q, _s = _add_rms_norm(x, residual, weight, eps, "add_rms_norm", normed=True, scales=None)
+    return total, normed
+
+
+def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6, *,
+                       scales: str = "1x128", backend: str = "cuda") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(total, q, scales): ``total = x + residual`` (x itself without a residual) and the e4m3 values of
+    ``rms_norm(total, weight, eps)``, quantised from fp32 without a 16-bit step between.
+
+    ``scales="1x128"``: fp32 [..., K / 128], amax / 448 of a 1 x 128 block: the operand of ``fp8_gemm``, as
+    ``quantize_activation_1x128`` writes it.  ``scales="mx"``: power-of-two scale atoms for ``mx_gemm``, as
+    ``quantize_activation_mx`` writes them.  The width is a multiple of 128, at most 16384.  Forward only:
+    ``add_rms_norm`` is the differentiable form."""
+    _require_backend_name("add_rms_norm_quant", backend)
+    if scales not in _SCALE_KINDS:
+        raise ValueError(f"unknown add_rms_norm_quant scales {scales}")
+    _refuse_autograd("add_rms_norm_quant", x, residual, weight)
+    if _TIMING is None:
+        fast = _host.add_rms_norm(x, residual, weight, eps, _SCALE_KINDS[scales])
+        if fast is not None:
+            return fast
+    total, _n, q, sc = _add_rms_norm(x, residual, weight, eps, "add_rms_norm_quant", normed=False, scales=scales)
+    return total, q, sc
+
+
+def add_rms_norm_backward(total: torch.Tensor, weight: torch.Tensor, grad_normed: torch.Tensor, grad_total: torch.Tensor | None = None,
+                          eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """(grad, dweight) of ``add_rms_norm``: ``grad`` is the gradient of x and of residual alike, from the upstream gradients of
+    ``normed`` and (None: zero) of ``total``.  Statistics recomputed from ``total`` in fp32; sums in a fixed order."""
+    if _TIMING is None:
+        fast = _host.add_rms_norm_backward(total, weight, grad_normed, grad_total, eps)
+        if fast is not None:
+            return fast
+    if grad_normed.shape != total.shape or (grad_total is not None and grad_total.shape != total.shape):
+        raise ValueError("add_rms_norm_backward needs gradients of total's shape")
+    matrix, _res, w = _normalize_add_rms_norm_inputs(total, None, weight, "add_rms_norm_backward", 8)
+    _require_cuda_tensors("cuda add_rms_norm_backward", total, grad_normed, grad_total)
+    dn = _aligned(grad_normed.reshape(matrix.shape).to(matrix.dtype))
+    dt = None if grad_total is None else _aligned(grad_total.reshape(matrix.shape).to(matrix.dtype))
+    grad, dw = torch.empty_like(matrix), torch.empty_like(w)
+    lib = _lib.load()
+    rows, cols = matrix.shape
+    work = torch.empty(int(lib.tb200_add_rmsnorm_bwd_workspace_bytes(cols)) // 4, dtype=torch.float32, device=matrix.device)
+    with torch.cuda.device(matrix.device), _timed("add_rms_norm_bwd", rows=rows, cols=cols, esize=matrix.element_size()):
+        code = lib.tb200_add_rmsnorm_bwd(_ptr(matrix), _ptr(w), _ptr(dn), _ptr(dt), _ptr(grad), _ptr(dw), _ptr(work), rows, cols, float(eps),
+                                         _DTYPE_CODES[matrix.dtype], _stream_ptr())
+    _lib.check(code, "cuda add_rms_norm_backward")
+    return grad.view(total.shape), dw
+
+
+class _AddRmsNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        ctx.set_materialize_grads(False)
+        with torch.no_grad():
+            total, normed = add_rms_norm(x, residual, weight, eps)
+        ctx.save_for_backward(total, weight)
+        ctx.eps = eps
+        return total, normed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_total, grad_normed):
+        total, weight = ctx.saved_tensors
+        if grad_normed is None:
+            return grad_total, grad_total, None, None
+        grad, dw = add_rms_norm_backward(total, weight, grad_normed, grad_total, ctx.eps)
+        return grad, grad, dw.to(weight.dtype), None
 
 
 # --------------------------------------------------------------------------------------------
@@ -1401,6 +1552,144 @@ def ffn_fp8(x: torch.Tensor, weights: Fp8FfnWeights, *, residual: torch.Tensor |
     y = fp8_gemm(h, sh, weights.w_down, weights.s_down, mode="linear", bias=weights.b_down, residual=res, check=check,
                  status=status)
     return y.view(*shape[:-1], weights.w_down.shape[0])
+
+
+# --------------------------------------------------------------------------------------------
+# activations kept in 8 bits for the backward pass
+# --------------------------------------------------------------------------------------------
+def _keep_operand(name: str, x: torch.Tensor, halves: int = 1) -> torch.Tensor:
+    if x.ndim < 1 or x.shape[-1] == 0 or x.shape[-1] % (128 * halves):
+        raise ValueError(f"{name} needs the last dimension to be a multiple of {128 * halves}")
+    _require_backend(name, "cuda")
+    _require_cuda_tensors(f"cuda {name}", x)
+    if x.dtype not in _DTYPE_CODES:
+        raise RuntimeError(f"cuda {name} does not support dtype {x.dtype}")
+    return _aligned(x.detach().reshape(-1, x.shape[-1]))
+
+
+def _kept_operand(name: str, q: torch.Tensor, scales: torch.Tensor, halves: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
+    if q.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise ValueError(f"{name} needs e4m3 values and fp32 scales")
+    if q.ndim < 1 or q.shape[-1] == 0 or q.shape[-1] % (128 * halves):
+        raise ValueError(f"{name} needs the last dimension to be a multiple of {128 * halves}")
+    if tuple(scales.shape) != (*q.shape[:-1], q.shape[-1] // 128):
+        raise ValueError(f"{name} scales must be [..., {q.shape[-1] // 128}] beside values [..., {q.shape[-1]}]")
+    _require_backend(name, "cuda")
+    _require_cuda_tensors(f"cuda {name}", q, scales)
+    return _aligned(q.reshape(-1, q.shape[-1])), scales.reshape(-1, scales.shape[-1]).contiguous()
+
+
+def checkpoint_activation(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """fp32 / fp16 / bf16 [..., K] -> (e4m3 [..., K], fp32 scales [..., K / 128]): what a layer keeps of an activation for its
+    backward pass, in a half or a quarter of the bytes.
+
+    The scale is the smallest power of two that brings a block's largest finite value to at most 448, so that
+    ``restore_activation`` rounds nothing, and the pair is an operand of ``fp8_gemm`` as it stands.  Values that are not
+    finite are kept as NaN."""
+    matrix = _keep_operand("checkpoint_activation", x)
+    rows, cols = matrix.shape
+    q = torch.empty(matrix.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty(rows, cols // 128, dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device), _timed("checkpoint_activation", rows=rows, cols=cols, esize=matrix.element_size()):
+        code = _lib.load().tb200_keep_fwd(_ptr(matrix), _ptr(q), _ptr(scales), rows, cols, _DTYPE_CODES[matrix.dtype], _stream_ptr())
+    _lib.check(code, "cuda checkpoint_activation")
+    return q.view(x.shape), scales.view(*x.shape[:-1], cols // 128)
+
+
+def restore_activation(q: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that ``checkpoint_activation`` kept, ``q * scale``, in ``dtype`` (exact in fp32 and bf16, and in fp16 in its range)."""
+    if dtype not in _DTYPE_CODES:
+        raise ValueError(f"restore_activation does not support dtype {dtype}")
+    matrix, s = _kept_operand("restore_activation", q, scales)
+    rows, cols = matrix.shape
+    out = torch.empty(matrix.shape, dtype=dtype, device=q.device)
+    with torch.cuda.device(q.device), _timed("restore_activation", rows=rows, cols=cols, esize=out.element_size()):
+        code = _lib.load().tb200_keep_restore(_ptr(matrix), _ptr(s), _ptr(out), rows, cols, _DTYPE_CODES[dtype], _stream_ptr())
+    _lib.check(code, "cuda restore_activation")
+    return out.view(q.shape)
+
+
+def _silu_gate(up: torch.Tensor, gated: bool, gate_first: bool, keep: bool, name: str):
+    if _TIMING is None:
+        fast = _host.silu_gate(up, gated, gate_first, keep)
+        if fast is not None:
+            return fast
+    matrix = _keep_operand(name, up, 2 if gated else 1)
+    rows, width = matrix.shape
+    hidden = width // 2 if gated else width
+    h = torch.empty(rows, hidden, dtype=matrix.dtype, device=up.device)
+    q = torch.empty(matrix.shape, dtype=torch.float8_e4m3fn, device=up.device) if keep else None
+    scales = torch.empty(rows, width // 128, dtype=torch.float32, device=up.device) if keep else None
+    with torch.cuda.device(up.device), _timed("silu_gate", rows=rows, cols=width, esize=matrix.element_size(), keep=keep):
+        code = _lib.load().tb200_silu_gate_fwd(_ptr(matrix), _ptr(h), _ptr(q), _ptr(scales), rows, hidden, int(bool(gated)), int(bool(gate_first)),
+                                               _DTYPE_CODES[matrix.dtype], _stream_ptr())
+    _lib.check(code, f"cuda {name}")
+    h = h.view(*up.shape[:-1], hidden)
+    return (h, q.view(up.shape), scales.view(*up.shape[:-1], width // 128)) if keep else h
+
+
+def silu_gate(up: torch.Tensor, *, gated: bool = True, gate_first: bool = True, backend: str = "cuda") -> torch.Tensor:
+    """The activation of a feed-forward layer: ``silu(gate) * value`` of ``up`` [..., 2 hidden] = [gate | value]
+    (``gate_first``, experiments/tokenformer/model.py:118-128) or [value | gate] (experiments/baseline/model.py:99-113);
+    ``gated=False``: ``silu(up)`` (experiments/onetrans/model.py:33-44).
+
+    Differentiable; what is kept for the backward pass is ``up`` in 8 bits (``silu_gate_checkpoint``), a rounding of half an
+    e4m3 step (2^-4) of each of its values that the gradient carries.  ``hidden`` is a multiple of 128."""
+    _require_backend_name("silu_gate", backend)
+    if torch.is_grad_enabled() and up.requires_grad:
+        return _SiluGateFunction.apply(up, bool(gated), bool(gate_first))
+    return _silu_gate(up, gated, gate_first, False, "silu_gate")
+
+
+def silu_gate_checkpoint(up: torch.Tensor, *, gated: bool = True, gate_first: bool = True
+                         ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(h, q, scales): ``silu_gate(up)`` and, from the same pass, ``checkpoint_activation(up)``."""
+    _refuse_autograd("silu_gate_checkpoint", up)
+    return _silu_gate(up, gated, gate_first, True, "silu_gate_checkpoint")
+
+
+def silu_gate_backward(q: torch.Tensor, scales: torch.Tensor, grad: torch.Tensor, *, gated: bool = True, gate_first: bool = True,
+                       activation: bool = True) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(grad_up, h): the gradient of ``silu_gate``'s input from what ``silu_gate_checkpoint`` kept and the gradient of its
+    result, and (``activation=True``) the activation of the kept values: the weight gradient of the layer behind it needs
+    it, and so nothing else has to be kept for that.  Both in ``grad``'s dtype."""
+    if _TIMING is None:
+        fast = _host.silu_gate_backward(q, scales, grad, gated, gate_first, activation)
+        if fast is not None:
+            return fast
+    matrix, s = _kept_operand("silu_gate_backward", q, scales, 2 if gated else 1)
+    rows, width = matrix.shape
+    hidden = width // 2 if gated else width
+    if tuple(grad.shape) != (*q.shape[:-1], hidden):
+        raise ValueError(f"silu_gate_backward grad must be {(*q.shape[:-1], hidden)}, got {tuple(grad.shape)}")
+    _require_cuda_tensors("cuda silu_gate_backward", q, grad)
+    if grad.dtype not in _DTYPE_CODES:
+        raise RuntimeError(f"cuda silu_gate_backward does not support dtype {grad.dtype}")
+    dh = _aligned(grad.detach().reshape(rows, hidden))
+    dup = torch.empty(rows, width, dtype=grad.dtype, device=q.device)
+    h = torch.empty_like(dh) if activation else None
+    with torch.cuda.device(q.device), _timed("silu_gate_bwd", rows=rows, cols=width, esize=dh.element_size()):
+        code = _lib.load().tb200_silu_gate_bwd(_ptr(matrix), _ptr(s), _ptr(dh), _ptr(dup), _ptr(h), rows, hidden, int(bool(gated)),
+                                               int(bool(gate_first)), _DTYPE_CODES[grad.dtype], _stream_ptr())
+    _lib.check(code, "cuda silu_gate_backward")
+    return dup.view(q.shape), None if h is None else h.view(grad.shape)
+
+
+class _SiluGateFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, up, gated, gate_first):
+        with torch.no_grad():
+            h, q, scales = silu_gate_checkpoint(up, gated=gated, gate_first=gate_first)
+        ctx.save_for_backward(q, scales)
+        ctx.form = (gated, gate_first)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, scales = ctx.saved_tensors
+        gated, gate_first = ctx.form
+        return silu_gate_backward(q, scales, grad, gated=gated, gate_first=gate_first, activation=False)[0], None, None
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, silu: bool = False,
