@@ -520,6 +520,28 @@ int tb200_join_summaries(const float* seq, const float* ns, float* joined, void*
 int tb200_head_fwd(const void* h, const float* w, const float* bias, float* logits, float* probs, int64_t batch, int32_t d, int32_t actions,
                    int dtype, void* stream);
 
+/* ---- linear layers grouped by expert with ragged sizes, and their gradients ---------------------
+ * The rows of x [T, K] lie expert by expert: rows offsets[e] .. offsets[e + 1] belong to expert e with the weights w[e] of
+ * [experts, N, K] (stacked `nn.Linear.weight`).  In the reference the parameter groups of a mixed layer: the sequence tokens
+ * share one set, every non-sequence token has its own (experiments/onetrans/model.py:47-107).
+ *     out[r] = act(x[r] @ w[e]^T + bias[e]) (+ residual[r]),   act: 0 = none, 1 = SiLU
+ * offsets: DEVICE int32 [experts + 1], read on the device; an offset outside [0, T] counts as the nearer end, one before an
+ * earlier offset as that one.  x, w, residual, out: fp16 or bf16 (dtype), contiguous; bias fp32 [experts, N]; bias and residual may be
+ * NULL; residual may be out itself.  Rows that belong to no expert are left as they are (clear = 0) or set to zero.
+ * N % 8 == 0, K % 8 == 0, experts <= 4096.  fp32 accumulation, one rounding.  status_word: as in tb200_gemm_bf16_grouped. */
+int tb200_ragged_gemm(const void* x, const void* w, const int32_t* offsets, const float* bias, const void* residual, void* out,
+                      int32_t experts, int64_t T, int32_t N, int32_t K, int32_t act, int32_t clear, int dtype,
+                      int32_t* status_word, void* stream);
+/* dx[r] = dy[r] @ w[e] of dy [T, N]; rows of no expert get zeros. */
+int tb200_ragged_gemm_dgrad(const void* dy, const void* w, const int32_t* offsets, void* dx, int32_t experts, int64_t T, int32_t N,
+                            int32_t K, int dtype, int32_t* status_word, void* stream);
+/* dw[e] = dy_e^T @ x_e ([experts, N, K], dtype) and db[e] = sum of the rows of dy_e (fp32 [experts, N]); either may be NULL (x
+ * too without dw); zeros for an expert without rows.  Rows of no expert are not looked at.  workspace: device memory of
+ * tb200_ragged_wgrad_workspace_bytes(...) bytes (on the current device), for this call alone.  The sums run in a fixed order. */
+int64_t tb200_ragged_wgrad_workspace_bytes(int32_t experts, int64_t T, int32_t N, int32_t K);
+int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int32_t* offsets, void* dw, float* db, float* workspace,
+                            int32_t experts, int64_t T, int32_t N, int32_t K, int dtype, int32_t* status_word, void* stream);
+
 /* ---- per-token (grouped) bf16 linear layers with a fused epilogue ----------------------------
  * out[g] = act(a[g] @ w[g]^T + bias[g]) (+ residual[g]) for g in [0, groups): the token-specific projections
  * and feed-forward layers of the non-sequence tokens, `nn.ModuleList` of `nn.Linear` / `FeedForward` applied

@@ -667,6 +667,92 @@ PyObject* py_silu_gate_backward(PyObject*, PyObject* const* args, Py_ssize_t) {
     END_HANDLE_TH_ERRORS
 }
 
+// -------------------------------------------------------------------------------------------- layers grouped by expert
+struct Ragged {
+    int64_t rows, n, k, experts;
+    int type;
+};
+// rows [T, width] against weight [E, N, K] (`width`: its dimension that the rows match) and int32 offsets [E + 1]
+bool ragged_operands(const Tensor& rows, const Tensor& w, const Tensor& off, int width, Ragged& r) {
+    const auto t = rows.scalar_type();
+    if (rows.dim() != 2 || w.dim() != 3 || off.dim() != 1 || (t != at::kBFloat16 && t != at::kHalf) || !plain(rows, t, rows) || !plain(w, t, rows) ||
+        !dense(off, at::kInt) || off.device() != rows.device() || off.size(0) != w.size(0) + 1 || rows.size(1) != w.size(width) ||
+        w.size(0) > INT32_MAX || w.size(1) > INT32_MAX || w.size(2) > INT32_MAX)
+        return false;
+    r = Ragged{rows.size(0), w.size(1), w.size(2), w.size(0), dtype_code(t)};
+    return true;
+}
+int32_t* status_at(const std::optional<Tensor>& status, const Tensor& beside, bool& ok) {
+    if (!status.has_value()) return nullptr;
+    ok = ok && status->scalar_type() == at::kInt && status->numel() == 1 && status->device() == beside.device();
+    return ok ? status->data_ptr<int32_t>() : nullptr;
+}
+
+// ragged_linear(x, weight, offsets, bias or None, silu, residual or None, out or None, status or None)
+PyObject* py_ragged_linear(PyObject*, PyObject* const* args, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    for (int i : {0, 1, 2})
+        if (!is_tensor(args[i])) Py_RETURN_NONE;
+    for (int i : {3, 5, 6, 7})
+        if (!is_optional(args[i])) Py_RETURN_NONE;
+    const Tensor& x = tensor(args[0]);
+    const Tensor& w = tensor(args[1]);
+    const Tensor& off = tensor(args[2]);
+    const auto bias = optional_tensor(args[3]), residual = optional_tensor(args[5]), into = optional_tensor(args[6]), status = optional_tensor(args[7]);
+    const bool silu = truth(args[4]);
+    Ragged r;
+    if (!ragged_operands(x, w, off, 2, r)) Py_RETURN_NONE;
+    if (bias.has_value() && (!plain(*bias, at::kFloat, x) || bias->dim() != 2 || bias->size(0) != r.experts || bias->size(1) != r.n)) Py_RETURN_NONE;
+    for (const auto* t : {&residual, &into})
+        if (t->has_value() && (!plain(**t, x.scalar_type(), x) || (*t)->dim() != 2 || (*t)->size(0) != r.rows || (*t)->size(1) != r.n)) Py_RETURN_NONE;
+    bool ok = true;
+    int32_t* word = status_at(status, x, ok);
+    if (!ok) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(x.device());
+    if (!tb200_device_ok()) Py_RETURN_NONE;
+    Tensor out = into.has_value() ? *into : at::empty({r.rows, r.n}, x.options().requires_grad(false));
+    if (tb200_ragged_gemm(ptr(x), ptr(w), off.data_ptr<int32_t>(), static_cast<float*>(ptr(bias)), ptr(residual), ptr(out),
+                          static_cast<int32_t>(r.experts), r.rows, static_cast<int32_t>(r.n), static_cast<int32_t>(r.k), silu, !into.has_value(), r.type,
+                          word, stream_of(x)) != TB200_OK)
+        Py_RETURN_NONE;
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// ragged_linear_backward(x, weight, offsets, grad_out, bias, status or None) -> (dx, dweight, dbias or None)
+PyObject* py_ragged_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    for (int i : {0, 1, 2, 3})
+        if (!is_tensor(args[i])) Py_RETURN_NONE;
+    if (!is_optional(args[5])) Py_RETURN_NONE;
+    const Tensor& x = tensor(args[0]);
+    const Tensor& w = tensor(args[1]);
+    const Tensor& off = tensor(args[2]);
+    const Tensor& dy = tensor(args[3]);
+    const bool bias = truth(args[4]);
+    const auto status = optional_tensor(args[5]);
+    Ragged r;
+    if (!ragged_operands(dy, w, off, 1, r) || !plain(x, dy.scalar_type(), dy) || x.dim() != 2 || x.size(0) != r.rows || x.size(1) != r.k) Py_RETURN_NONE;
+    bool ok = true;
+    int32_t* word = status_at(status, x, ok);
+    if (!ok) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard guard(x.device());
+    if (!tb200_device_ok()) Py_RETURN_NONE;
+    const auto e = static_cast<int32_t>(r.experts), n = static_cast<int32_t>(r.n), k = static_cast<int32_t>(r.k);
+    const auto opt = x.options().requires_grad(false);
+    Tensor dx = at::empty(x.sizes(), opt), dw = at::empty(w.sizes(), opt), db;
+    if (bias) db = at::empty({r.experts, r.n}, opt.dtype(at::kFloat));
+    Tensor work = at::empty({std::max<int64_t>(tb200_ragged_wgrad_workspace_bytes(e, r.rows, n, k) / 4, 1)}, opt.dtype(at::kFloat));
+    const auto* offsets = off.data_ptr<int32_t>();
+    int code = tb200_ragged_gemm_dgrad(ptr(dy), ptr(w), offsets, ptr(dx), e, r.rows, n, k, r.type, word, stream_of(x));
+    if (code == TB200_OK)
+        code = tb200_ragged_gemm_wgrad(ptr(x), ptr(dy), offsets, ptr(dw), bias ? static_cast<float*>(ptr(db)) : nullptr, static_cast<float*>(ptr(work)), e,
+                                       r.rows, n, k, r.type, word, stream_of(x));
+    if (code != TB200_OK) Py_RETURN_NONE;
+    return tuple_of(dx, dw, db);
+    END_HANDLE_TH_ERRORS
+}
+
 #define TB200_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     TB200_METHOD(rms_norm),
@@ -682,6 +768,8 @@ PyMethodDef methods[] = {
     TB200_METHOD(add_rms_norm_backward),
     TB200_METHOD(silu_gate),
     TB200_METHOD(silu_gate_backward),
+    TB200_METHOD(ragged_linear),
+    TB200_METHOD(ragged_linear_backward),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Host side of the operator calls.", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,834 @@
+// Matrix products grouped by expert with ragged sizes, and their gradients, for sm_100a.  The rows of x [T, K] lie expert by
+// expert: expert e owns the rows offsets[e] .. offsets[e + 1] and has weights w[e] [N, K] of its own.
+//
+//   rows       out[r] = act(x[r] w[e]^T + bias[e]) (+ residual[r])                 r a row of e
+//   row grads  dx[r]  = dy[r] w[e]
+//   weights    dw[e]  = sum over the rows r of e of dy[r]^T x[r],     db[e] = sum of dy[r]
+//
+// The offsets are read on the device, so that a router's result needs no copy to the host.  They are clamped to [0, T] and
+// to what came before them: whatever they hold, nothing outside the tensors is touched and no row is computed twice.
+//
+// `ragged_pair_kernel` serves all three on clusters of two CTAs with 256 x 256 tiles, tcgen05 cta_group::2 and fp32 accumulation
+// in tensor memory: warp 0 of each CTA feeds a ring of TMA stages, warp 1 of the leader issues the MMAs, eight epilogue warps
+// work a tile behind on the other half of the accumulator.  What differs is which dimension is contracted:
+//   rows       both operands have the contraction innermost (K-major), as they lie in memory;
+//   row grads  w[e] is contracted over its rows: boxes of 64 contraction rows x 64 columns, the MN-major form of the operand;
+//   weights    both operands are contracted over the expert's rows, both MN-major.  The last block of an expert reaches into
+//              the next one's rows: these are set to zero in shared memory, in both operands (0 x NaN is NaN), before
+//              the MMAs see them.
+// A row tile that crosses its expert's end computes rows of the next expert for nothing and does not store them.
+//
+// Distribution.  Row tiles go round robin over the pairs.  The weight gradient of uneven experts does not: its tiles
+// differ in length, so all tiles' 64-row blocks are lined up and every pair takes an equal share of the line; a tile that
+// two or more pairs share leaves fp32 partial tiles in a workspace, which `ragged_join_kernel` adds in the order of the
+// pairs.  Shares that would leave less than kSnap blocks of a tile move to the tile's edge: writing and reading a partial tile costs
+// about as much as that many blocks.
+//
+// Every wait on an mbarrier is bounded; a wait that gives up raises the status word and all roles drain through the final barrier.
+#include "tb200_common.cuh"
+#include "tb200_tmap.cuh"
+#include "tc_pair.cuh"
+
+namespace tb200 {
+void count_launch();
+
+namespace {
+
+enum Mode : int { kRows = 0, kRowGrads = 1, kWeights = 2 };
+
+constexpr int kTile = 256;                                // of a pair, both ways; a CTA holds 128 of its rows
+constexpr int kBlock = 64;                                // contracted per stage: 128 bytes of a 16-bit type, or 64 rows
+constexpr uint32_t kOperandBytes = 128 * 128;             // one CTA's half of an operand in a stage
+constexpr uint32_t kStageBytes = 2 * kOperandBytes;
+constexpr uint32_t kChunkBytes = 64 * 128;                // MN-major: 64 contraction rows x 128 bytes
+constexpr int kMaxStages = 6;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + kEpiWarps * 32;
+constexpr uint32_t kBoxBytes = 32 * 128;                  // an epilogue warp's staging box: 32 rows x 64 columns
+constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxExperts = 4096;
+constexpr int kSnap = 8;
+constexpr int64_t kPartFloats = int64_t(kTile) * kTile;   // of a partial tile
+constexpr size_t kSmemLimit = 227 * 1024 - 512;           // less the static part
+
+struct RaggedArgs {
+    const int32_t* offsets;     // [experts + 1]
+    const float* bias;          // [experts, cols] or NULL (rows)
+    const void* residual;       // [T, cols] or NULL (rows)
+    void* out;                  // [T, cols], or [experts, n, k] (weights)
+    float* partial;             // [pairs][2] partial tiles, NULL: tiles are never shared (weights)
+    int32_t* status;
+    int32_t experts, stages;
+    int64_t T;
+    int32_t cols;               // of a result row
+    int32_t depth;              // contracted length (rows, row grads)
+    int32_t n;                  // rows of a weight gradient
+    int32_t silu;
+    int32_t clear;              // rows of no expert are set to zero
+};
+
+// Units of work of `rows` rows: row tiles, 64-row blocks (an expert without rows has one: the zeros of its weight gradient are
+// written), or the pieces of the bias gradient
+enum Units : int { kTiles, kBlocks, kBiasPieces };
+constexpr int kBiasRows = 256;
+template <int U>
+__device__ __forceinline__ int units_of(int rows) {
+    if (U == kTiles) return (rows + kTile - 1) / kTile;
+    if (U == kBlocks) return rows == 0 ? 1 : (rows + kBlock - 1) / kBlock;
+    return (rows + kBiasRows - 1) / kBiasRows;
+}
+// Where every expert's rows begin, and how many units the experts before it have.  An offset outside [0, T] is moved to
+// the nearer end and one that lies before an earlier one counts as that one, so that no two experts share a row.
+struct Plan {
+    int32_t* begin;    // [experts + 1] in shared memory
+    int32_t* pre;      // [experts + 1]
+};
+__device__ __forceinline__ Plan plan_at(void* smem, int experts) {
+    int32_t* p = static_cast<int32_t*>(smem);
+    return Plan{p, p + experts + 1};
+}
+// By one warp; the offsets come from the kernel in front.
+template <int U>
+__device__ void make_plan(const RaggedArgs& g, const Plan& plan, int lane) {
+    int32_t top = 0;
+    for (int base = 0; base <= g.experts; base += 32) {
+        int32_t v = 0;
+        if (base + lane <= g.experts) v = __ldcg(g.offsets + base + lane);
+        v = v < 0 ? 0 : (v > g.T ? static_cast<int32_t>(g.T) : v);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v = max(v, u);
+        }
+        v = max(v, top);
+        if (base + lane <= g.experts) plan.begin[base + lane] = v;
+        top = __shfl_sync(0xffffffffu, v, 31);
+    }
+    __syncwarp();
+    int32_t sum = 0;
+    for (int base = 0; base < g.experts; base += 32) {
+        const int e = base + lane;
+        int32_t v = e < g.experts ? units_of<U>(plan.begin[e + 1] - plan.begin[e]) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        if (e < g.experts) plan.pre[e + 1] = sum + v;
+        sum += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) plan.pre[0] = 0;
+}
+// the expert whose units hold `unit`
+__device__ __forceinline__ int expert_of(const int32_t* pre, int experts, int64_t unit) {
+    int lo = 0, hi = experts;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= unit) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+// Begin of pair i's share of the line of blocks, moved to the edge of its tile where it lies near one
+__device__ __forceinline__ int64_t share_begin(const int32_t* pre, int experts, int tiles, int i, int pairs, bool split) {
+    const int64_t total = static_cast<int64_t>(pre[experts]) * tiles;
+    if (i >= pairs) return total;
+    const int64_t p = total / pairs * i + total % pairs * i / pairs;
+    const int e = expert_of(pre, experts, p / tiles);
+    const int64_t base = static_cast<int64_t>(pre[e]) * tiles;
+    const int64_t nb = pre[e + 1] - pre[e];
+    if (nb == 0) return p;
+    const int64_t o = (p - base) % nb, begin = p - o;
+    if (!split) return 2 * o < nb ? begin : begin + nb;
+    return o < kSnap ? begin : (nb - o < kSnap ? begin + nb : p);
+}
+
+// One piece of a pair's work
+struct Job {
+    int e;
+    int64_t begin, end;        // the expert's rows
+    int64_t m0;                // rows: first row of the tile; weights: first row of the expert that is contracted
+    int32_t a0, b0;            // weights: first dw row and column; rows: b0 = first column of the tile
+    int blocks;                // stages of this piece
+    int slot;                  // weights: partial tile that receives it, -1: the whole tile
+};
+
+template <int MODE>
+struct Walk {
+    const RaggedArgs& g;
+    const int32_t *first_row, *pre;
+    int n_tiles, b_tiles;
+    int64_t at, stop, step;
+    int e = -1;
+    int64_t begin = 0, end = 0;
+
+    __device__ Walk(const RaggedArgs& args, const Plan& plan, int pair, int pairs) : g(args), first_row(plan.begin), pre(plan.pre) {
+        b_tiles = (g.cols + kTile - 1) / kTile;
+        n_tiles = MODE == kWeights ? (g.n + kTile - 1) / kTile : 1;
+        if (MODE == kWeights) {
+            at = share_begin(pre, g.experts, n_tiles * b_tiles, pair, pairs, g.partial != nullptr);
+            stop = share_begin(pre, g.experts, n_tiles * b_tiles, pair + 1, pairs, g.partial != nullptr);
+            step = 0;
+        } else {
+            at = pair;
+            stop = static_cast<int64_t>(pre[g.experts]) * b_tiles;
+            step = pairs;
+        }
+    }
+    __device__ bool next(Job& j) {
+        if (at >= stop) return false;
+        const int per = n_tiles * b_tiles;
+        const int64_t unit = at / per;
+        if (e < 0 || unit >= pre[e + 1]) {
+            e = e < 0 ? expert_of(pre, g.experts, unit) : e + 1;
+            while (unit >= pre[e + 1]) ++e;
+            begin = first_row[e];
+            end = first_row[e + 1];
+        }
+        j.e = e;
+        j.begin = begin;
+        j.end = end;
+        if (MODE == kWeights) {
+            const int nb = pre[e + 1] - pre[e];
+            const int64_t local = at - static_cast<int64_t>(pre[e]) * per;
+            const int tile = static_cast<int>(local / nb), first = static_cast<int>(local % nb);
+            const int64_t left = stop - at;
+            const int take = left < nb - first ? static_cast<int>(left) : nb - first;
+            j.a0 = tile / b_tiles * kTile;
+            j.b0 = tile % b_tiles * kTile;
+            j.m0 = begin + static_cast<int64_t>(first) * kBlock;
+            j.blocks = end > begin ? take : 0;
+            j.slot = take == nb ? -1 : (first > 0 ? 0 : 1);
+            at += take;
+        } else {
+            j.b0 = static_cast<int>(at % b_tiles) * kTile;
+            j.a0 = 0;
+            j.m0 = begin + (unit - pre[e]) * kTile;
+            j.blocks = (g.depth + kBlock - 1) / kBlock;
+            j.slot = -1;
+            at += step;
+        }
+        return true;
+    }
+};
+
+// silu(x) = x / (1 + exp(-x))
+__device__ __forceinline__ float silu(float x) { return x * __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+// Sets the contraction rows [valid, 64) of a stage's four chunks to zero, by one warp
+__device__ __forceinline__ void clear_tail(uint8_t* stage, int valid, int lane) {
+    const int pieces = (kBlock - valid) * 8;
+    for (int i = lane; i < 4 * pieces; i += 32) {
+        const int chunk = i / pieces, r = i - chunk * pieces;
+        *reinterpret_cast<uint4*>(stage + chunk * kChunkBytes + valid * 128 + r * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+template <typename T, int MODE, bool RES>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                   const __grid_constant__ CUtensorMap tmap_o, const RaggedArgs g) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full_bar[kMaxStages];     // used in the leader only
+    __shared__ uint64_t empty_bar[kMaxStages];
+    __shared__ uint64_t tail_bar[kMaxStages];     // weights, the other CTA: its own loads of an expert's last block
+    __shared__ uint64_t tmem_full[2];
+    __shared__ uint64_t tmem_empty[2];            // used in the leader only
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int s_abort;
+
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* out_s = ring + static_cast<size_t>(g.stages) * kStageBytes;
+    const Plan plan = plan_at(out_s + kEpiWarps * kBoxBytes, g.experts);
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();         // 0 = leader
+    const int pair = blockIdx.x >> 1;
+    const int pairs = gridDim.x >> 1;
+    constexpr bool kFmtBf16 = std::is_same<T, __nv_bfloat16>::value;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < g.stages; ++s) {
+            mbar_init(&full_bar[s], MODE == kWeights ? 2 : 1);
+            mbar_init(&empty_bar[s], 1);
+            mbar_init(&tail_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tmem_full[b], 1);
+            mbar_init(&tmem_empty[b], 2 * kEpiWarps);
+        }
+        s_abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc_pair(&tmem_base_slot, kTmemCols);
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();                           // both CTAs' barriers exist before anything is signalled remotely
+    tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_base_slot;
+    chain_release();                              // not before every CTA holds its tensor memory (see launch_chained)
+    chain_wait();
+    if (warp == 0) make_plan<MODE == kWeights ? kBlocks : kTiles>(g, plan, lane);
+    __syncthreads();
+
+    Walk<MODE> walk(g, plan, pair, pairs);
+    Job j;
+    if (warp == 0) {
+        // ---------------------------------------------------------------- TMA producer (both CTAs)
+        if (lane == 0) {
+            tma_prefetch_desc(&tmap_a);
+            tma_prefetch_desc(&tmap_b);
+            uint32_t s = 0, ph = 0;
+            bool ok = true;
+            while (ok && walk.next(j)) {
+                for (int b = 0; b < j.blocks; ++b) {
+                    if (!mbar_wait_sleep(&empty_bar[s], ph ^ 1) || *reinterpret_cast<volatile int*>(&s_abort)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* dst = ring + static_cast<size_t>(s) * kStageBytes;
+                    if (MODE == kWeights) {
+                        const int64_t row = j.m0 + static_cast<int64_t>(b) * kBlock;
+                        const int32_t y = static_cast<int32_t>(row);
+                        const int32_t xa = (j.a0 + static_cast<int>(rank) * 128) * 2, xb = (j.b0 + static_cast<int>(rank) * 128) * 2;
+                        if (row + kBlock > j.end && rank != 0) {     // this CTA's warp 1 clears the rows behind the end and then tells the leader
+                            mbar_expect_tx(&tail_bar[s], kStageBytes);
+                            tma_load_2d(dst, &tmap_a, xa, y, &tail_bar[s]);
+                            tma_load_2d(dst + kChunkBytes, &tmap_a, xa + 128, y, &tail_bar[s]);
+                            tma_load_2d(dst + 2 * kChunkBytes, &tmap_b, xb, y, &tail_bar[s]);
+                            tma_load_2d(dst + 3 * kChunkBytes, &tmap_b, xb + 128, y, &tail_bar[s]);
+                        } else {
+                            if (rank == 0) {
+                                const bool tail = row + kBlock > j.end;
+                                mbar_expect_tx(&full_bar[s], tail ? kStageBytes : 2 * kStageBytes);
+                                if (!tail) mbar_arrive(&full_bar[s]);
+                            }
+                            tma_load_2d_pair(dst, &tmap_a, xa, y, &full_bar[s]);
+                            tma_load_2d_pair(dst + kChunkBytes, &tmap_a, xa + 128, y, &full_bar[s]);
+                            tma_load_2d_pair(dst + 2 * kChunkBytes, &tmap_b, xb, y, &full_bar[s]);
+                            tma_load_2d_pair(dst + 3 * kChunkBytes, &tmap_b, xb + 128, y, &full_bar[s]);
+                        }
+                    } else {
+                        if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);   // the bytes of both CTAs
+                        tma_load_2d_pair(dst, &tmap_a, b * 128, static_cast<int32_t>(j.m0) + static_cast<int>(rank) * 128, &full_bar[s]);
+                        const int32_t col = j.b0 + static_cast<int>(rank) * 128;
+                        if (MODE == kRows) {
+                            tma_load_3d_pair(dst + kOperandBytes, &tmap_b, b * 128, col, j.e, &full_bar[s]);
+                        } else {
+                            tma_load_3d_pair(dst + kOperandBytes, &tmap_b, col * 2, b * kBlock, j.e, &full_bar[s]);
+                            tma_load_3d_pair(dst + kOperandBytes + kChunkBytes, &tmap_b, col * 2 + 128, b * kBlock, j.e, &full_bar[s]);
+                        }
+                    }
+                    if (++s == static_cast<uint32_t>(g.stages)) {
+                        s = 0;
+                        ph ^= 1;
+                    }
+                }
+            }
+            if (!ok) {
+                s_abort = 1;
+                if (g.status != nullptr) atomicExch(g.status, 1);
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            // ------------------------------------------------------------ MMA issuer (leader; an elected lane issues, see mbar_wait_warp)
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            constexpr uint32_t fmt = kFmtBf16 ? 1 : 0;
+            const uint32_t idesc = umma_idesc(fmt, fmt, MODE == kWeights ? 1 : 0, MODE == kRows ? 0 : 1, kTile, kTile);
+            // K-major: groups of 8 rows are 1024 bytes apart, 16 elements further along K are 32 bytes.  MN-major: groups of 8
+            // contraction rows are 1024 bytes apart, the next 64 columns are a chunk further, 16 contraction rows are 2048 bytes.
+            const uint64_t desc_k = umma_desc_sw128(0, 1024, 16), desc_mn = umma_desc_sw128(0, 1024, kChunkBytes);
+            const uint64_t da0 = MODE == kWeights ? desc_mn : desc_k, db0 = MODE == kRows ? desc_k : desc_mn;
+            constexpr int step_a = MODE == kWeights ? 128 : 2, step_b = MODE == kRows ? 2 : 128;
+            const uint32_t ring_lo = (smem_u32(ring) & 0x3FFFFu) >> 4;
+            uint32_t s = 0, ph = 0, buf = 0, aph = 0;
+            bool ok = true;
+            while (ok && walk.next(j)) {
+                if (MODE == kWeights && j.blocks == 0) continue;
+                if (!mbar_wait_warp(&tmem_empty[buf], aph ^ 1)) { ok = false; break; }
+                tc_fence_after_sync();
+                const uint32_t d_tmem = tmem + buf * kTile;
+                for (int b = 0; b < j.blocks; ++b) {
+                    if (!mbar_wait_warp(&full_bar[s], ph)) { ok = false; break; }
+                    if (MODE == kWeights) {
+                        const int64_t valid = j.end - (j.m0 + static_cast<int64_t>(b) * kBlock);
+                        if (valid < kBlock) {
+                            asm volatile("fence.acq_rel.cluster;" ::: "memory");      // the other CTA has cleared its half
+                            clear_tail(ring + static_cast<size_t>(s) * kStageBytes, static_cast<int>(valid), lane);
+                        }
+                    }
+                    tc_fence_after_sync();
+                    const uint64_t da = da0 + ring_lo + s * (kStageBytes >> 4);
+                    const uint64_t db = db0 + ring_lo + s * (kStageBytes >> 4) + (kOperandBytes >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < kBlock / 16; ++k)
+                            mma_f16_ss_pair(d_tmem, da + step_a * k, db + step_b * k, idesc, (b | k) != 0 ? 1u : 0u);
+                        tc_commit_pair(&empty_bar[s]);
+                    }
+                    __syncwarp();
+                    if (++s == static_cast<uint32_t>(g.stages)) {
+                        s = 0;
+                        ph ^= 1;
+                    }
+                }
+                if (!ok) break;
+                if (elect_one()) tc_commit_pair(&tmem_full[buf]);
+                __syncwarp();
+                aph ^= buf;
+                buf ^= 1;
+            }
+            if (!ok) {
+                s_abort = 1;
+                if (g.status != nullptr) atomicExch(g.status, 1);
+            }
+        } else if (MODE == kWeights) {
+            // ------------------------------------------------------------ the other CTA's last blocks
+            uint32_t s = 0, tail_ph = 0;
+            bool ok = true;
+            while (ok && walk.next(j)) {
+                for (int b = 0; b < j.blocks; ++b) {
+                    const int64_t valid = j.end - (j.m0 + static_cast<int64_t>(b) * kBlock);
+                    if (valid < kBlock) {
+                        if (!mbar_wait_warp(&tail_bar[s], (tail_ph >> s) & 1)) { ok = false; break; }
+                        tail_ph ^= 1u << s;
+                        clear_tail(ring + static_cast<size_t>(s) * kStageBytes, static_cast<int>(valid), lane);
+                        if (lane == 0) mbar_arrive_leader_release(&full_bar[s]);
+                        __syncwarp();
+                    }
+                    if (++s == static_cast<uint32_t>(g.stages)) s = 0;
+                }
+            }
+            if (!ok) {
+                s_abort = 1;
+                if (g.status != nullptr) atomicExch(g.status, 1);
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- epilogue (both CTAs, own 128 rows)
+        // A warp owns the 32 rows of its TMEM lane quarter and 128 of the tile's 256 columns, in two units of 64: 32 columns at a
+        // time from TMEM, bias / activation / residual, rounded into a private 4 KB box (128-byte swizzle), one TMA store a
+        // unit.  The tensor map clips columns; rows behind the expert's end must stay as they are, so a box that reaches
+        // behind it is written by plain stores instead, each lane its own row.
+        const int ew = warp - 2;
+        const int half = ew >> 2;
+        const int quarter = warp & 3;             // TMEM lanes [32 quarter, +32) are the ones this warp may read
+        const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+        uint8_t* box = out_s + ew * kBoxBytes;
+        const int swz = lane & 7;
+        T* out = static_cast<T*>(g.out);
+        if (MODE != kWeights && g.clear) {        // rows in front of the first expert and behind the last
+            const int64_t head = plan.begin[0], owned = plan.begin[g.experts] - head;
+            const int64_t row_pieces = g.cols / 8, pieces = (g.T - owned) * row_pieces;
+            for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kEpiWarps * 32) + threadIdx.x - 64; i < pieces;
+                 i += static_cast<int64_t>(gridDim.x) * (kEpiWarps * 32)) {
+                int64_t r = i / row_pieces;
+                const int64_t c = i - r * row_pieces;
+                if (r >= head) r += owned;
+                reinterpret_cast<uint4*>(out)[r * row_pieces + c] = make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+        uint32_t buf = 0, aph = 0;
+        bool ok = true;
+        while (walk.next(j)) {
+            const bool none = MODE == kWeights && j.blocks == 0;      // zeros, without the tensor cores
+            const int64_t row0 = MODE == kWeights ? j.a0 + static_cast<int>(rank) * 128 + quarter * 32
+                                                  : j.m0 + static_cast<int>(rank) * 128 + quarter * 32;
+            const int64_t row = row0 + lane;
+            const int64_t row_end = MODE == kWeights ? g.n : j.end;
+            const bool boxed = MODE == kWeights || row0 + 32 <= row_end;
+            const bool live = row < row_end;
+            const int col0 = j.b0 + half * 128;
+            const float* bias_t = MODE == kRows && g.bias != nullptr ? g.bias + static_cast<int64_t>(j.e) * g.cols : nullptr;
+            const T* res_row = RES ? static_cast<const T*>(g.residual) + row * g.cols : nullptr;
+            float* part = nullptr;
+            if (MODE == kWeights && j.slot >= 0)
+                part = g.partial + (static_cast<int64_t>(pair) * 2 + j.slot) * kPartFloats + static_cast<int64_t>(rank) * (kPartFloats / 2) +
+                       (quarter * 32 + lane) * 4;
+            // A warp whose wait gives up stops waiting but keeps walking (it still arrives on the accumulator barrier).
+            if (ok && !none) {
+                int passed = 1;
+                if (lane == 0) passed = mbar_wait_sleep(&tmem_full[buf], aph) ? 1 : 0;
+                if (__shfl_sync(0xffffffffu, passed, 0) == 0) ok = false;
+            }
+            tc_fence_after_sync();
+#pragma unroll 1
+            for (int piece = 0; piece < 4; ++piece) {              // 32 accumulator columns each, two of them a box
+                const int sub = piece & 1;
+                const int col = col0 + piece * 32;
+                uint32_t acc[32];
+                uint4 res[RES ? 4 : 1];
+                if (RES) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        res[RES ? q : 0] = live && col + q * 8 < g.cols ? *reinterpret_cast<const uint4*>(res_row + col + q * 8) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                if (!none) {
+                    tmem_ld_2x16(tmem_base + buf * kTile + lane_addr + half * 128 + piece * 32, acc);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[i] = 0u;
+                }
+                if (sub == 0 && lane == 0) bulk_wait_read<0>();    // this warp's previous store has read the box
+                if (!none) tc_wait_ld(acc);
+                if (piece == 3 && !none) {                         // the warp holds its share in registers: hand the buffer back
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_leader(&tmem_empty[buf]);
+                } else {
+                    __syncwarp();
+                }
+                if (MODE == kWeights && part != nullptr) {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        *reinterpret_cast<uint4*>(part + static_cast<int64_t>(half * 32 + piece * 8 + q) * 512) =
+                            make_uint4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+                    continue;
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int c = col + q * 8;
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(acc[8 * q + e]);
+                    if (MODE == kRows) {
+                        if (bias_t != nullptr && c < g.cols) {
+                            const float4 b0 = __ldg(reinterpret_cast<const float4*>(bias_t + c)), b1 = __ldg(reinterpret_cast<const float4*>(bias_t + c + 4));
+                            v[0] += b0.x; v[1] += b0.y; v[2] += b0.z; v[3] += b0.w;
+                            v[4] += b1.x; v[5] += b1.y; v[6] += b1.z; v[7] += b1.w;
+                        }
+                        if (g.silu) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] = silu(v[e]);
+                        }
+                        if (RES) {
+                            float r[8];
+                            Vec16<T>::unpack(res[RES ? q : 0], r);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] += r[e];
+                        }
+                    }
+                    const uint4 w = Vec16<T>::pack(v);
+                    if (boxed) *reinterpret_cast<uint4*>(box + lane * 128 + (((sub * 4 + q) ^ swz) << 4)) = w;
+                    else if (live && c < g.cols) *reinterpret_cast<uint4*>(out + row * g.cols + c) = w;
+                }
+                if (sub == 1 && boxed) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    const int cbox = col0 + (piece >> 1) * 64;
+                    if (lane == 0 && cbox < g.cols && row0 < row_end) {
+                        if (MODE == kWeights) tma_store_3d(&tmap_o, box, cbox * 2, static_cast<int32_t>(row0), j.e);
+                        else tma_store_2d(&tmap_o, box, cbox * 2, static_cast<int32_t>(row0));
+                        bulk_commit();
+                    }
+                }
+            }
+            if (!none) {
+                aph ^= buf;
+                buf ^= 1;
+            }
+        }
+        if (lane == 0) bulk_wait<0>();            // the last store must have left shared memory before the CTA ends
+        if (!ok) {
+            s_abort = 1;
+            if (g.status != nullptr) atomicExch(g.status, 1);
+        }
+    }
+
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();                           // the peer may still read this CTA's shared memory or signal its barriers
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+}
+
+// Adds the partial tiles of every shared weight-gradient tile.  CTA x of column y looks at the border between the shares of pairs x and
+// x + 1: if it lies inside a tile and is the first to do so, the CTA adds what the pairs left there, in their order, for 32 of
+// the tile's columns (a thread holds one of the 256 rows).
+template <typename T>
+__global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, int pairs) {
+    extern __shared__ int32_t plan_s[];
+    const Plan plan = plan_at(plan_s, g.experts);
+    const int32_t* pre = plan.pre;
+    chain_release();
+    chain_wait();
+    if (threadIdx.x < 32) make_plan<kBlocks>(g, plan, threadIdx.x);
+    __syncthreads();
+    const int b_tiles = (g.cols + kTile - 1) / kTile, tiles = (g.n + kTile - 1) / kTile * b_tiles;
+    const int i = blockIdx.x + 1;
+    const int64_t p = share_begin(pre, g.experts, tiles, i, pairs, true), total = static_cast<int64_t>(pre[g.experts]) * tiles;
+    if (p >= total) return;
+    const int e = expert_of(pre, g.experts, p / tiles);
+    const int64_t base = static_cast<int64_t>(pre[e]) * tiles, nb = pre[e + 1] - pre[e];
+    const int64_t begin = p - (p - base) % nb, end = begin + nb;
+    if (p == begin || share_begin(pre, g.experts, tiles, i - 1, pairs, true) > begin) return;
+    const int tile = static_cast<int>((begin - base) / nb);
+    const int r = threadIdx.x;
+    const int row = tile / b_tiles * kTile + r, col = tile % b_tiles * kTile + blockIdx.y * 32;
+    float4 sum[8];
+    auto add = [&](int pair, int slot, bool first) {
+        const float* part = g.partial + (static_cast<int64_t>(pair) * 2 + slot) * kPartFloats + (r >> 7) * (kPartFloats / 2) + (r & 127) * 4;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + static_cast<int64_t>(blockIdx.y * 8 + q) * 512));
+            if (first) sum[q] = v;
+            else sum[q] = make_float4(sum[q].x + v.x, sum[q].y + v.y, sum[q].z + v.z, sum[q].w + v.w);
+        }
+    };
+    add(i - 1, 1, true);
+    int64_t lo = p;
+    for (int k = i; k < pairs && lo < end; ++k) {
+        const int64_t hi = share_begin(pre, g.experts, tiles, k + 1, pairs, true);
+        if (hi > lo) add(k, 0, false);
+        lo = hi;
+    }
+    if (row >= g.n) return;
+    T* out = static_cast<T*>(g.out) + (static_cast<int64_t>(e) * g.n + row) * g.cols;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (col + q * 8 >= g.cols) break;
+        const float4 a = sum[2 * q], b = sum[2 * q + 1];
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        *reinterpret_cast<uint4*>(out + col + q * 8) = Vec16<T>::pack(v);
+    }
+}
+
+// db[e] = sum of the expert's rows of dy, in two steps of fixed order.  Step one: CTA (x, y) adds up to kBiasRows rows (a piece of
+// one expert) for 256 columns; its eight warps take every eighth row, eight columns a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) ragged_bias_part_kernel(const T* __restrict__ dy, const RaggedArgs g, float* __restrict__ part, int max_pieces) {
+    extern __shared__ int32_t plan_s[];
+    __shared__ float sums[8][256];
+    const Plan plan = plan_at(plan_s, g.experts);
+    const int32_t* pre = plan.pre;
+    chain_release();
+    chain_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 0) make_plan<kBiasPieces>(g, plan, lane);
+    __syncthreads();
+    const int piece = blockIdx.x;
+    if (piece >= pre[g.experts] || piece >= max_pieces) return;
+    const int e = expert_of(pre, g.experts, piece);
+    const int64_t first = plan.begin[e] + static_cast<int64_t>(piece - pre[e]) * kBiasRows, end = plan.begin[e + 1];
+    const int64_t last = first + kBiasRows < end ? first + kBiasRows : end;
+    const int col = blockIdx.y * 256 + lane * 8;
+    float acc[8] = {};
+    if (col < g.n) {
+#pragma unroll 4
+        for (int64_t r = first + warp; r < last; r += 8) {
+            float v[8];
+            Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4*>(dy + r * g.n + col)), v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] += v[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[warp][lane * 8 + i] = acc[i];
+    __syncthreads();
+    const int c = blockIdx.y * 256 + threadIdx.x;
+    if (c >= g.n) return;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += sums[k][threadIdx.x];
+    part[static_cast<int64_t>(piece) * g.n + c] = s;
+}
+
+__global__ void __launch_bounds__(256) ragged_bias_sum_kernel(const RaggedArgs g, const float* __restrict__ part, float* __restrict__ db, int max_pieces) {
+    extern __shared__ int32_t plan_s[];
+    const Plan plan = plan_at(plan_s, g.experts);
+    const int32_t* pre = plan.pre;
+    chain_release();
+    chain_wait();
+    if (threadIdx.x < 32) make_plan<kBiasPieces>(g, plan, threadIdx.x);
+    __syncthreads();
+    const int e = blockIdx.x;
+    const int c = blockIdx.y * 256 + threadIdx.x;
+    if (c >= g.n) return;
+    float s = 0.f;
+    const int last = min(pre[e + 1], max_pieces);
+#pragma unroll 4
+    for (int p = pre[e]; p < last; ++p) s += part[static_cast<int64_t>(p) * g.n + c];
+    db[static_cast<int64_t>(e) * g.n + c] = s;
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+// a matrix or a stack of matrices of 16-bit values, boxes of box_rows x 128 bytes
+bool make_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t stack, uint32_t box_rows) {
+    const auto fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[3] = {2 * cols, rows, stack};
+    const cuuint64_t strides[2] = {2 * cols, 2 * cols * rows};
+    const cuuint32_t box[3] = {128, box_rows, 1};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, stack == 0 ? 2 : 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int pairs_here() { return device_info().sm_count / 2; }
+
+size_t smem_of(int stages, int experts) {
+    return 1024 + static_cast<size_t>(stages) * kStageBytes + kEpiWarps * kBoxBytes + (static_cast<size_t>(experts) + 1) * 8;
+}
+
+template <typename T, int MODE, bool RES>
+int launch_pairs(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, RaggedArgs g, int pairs, cudaStream_t st) {
+    g.stages = kMaxStages;
+    while (smem_of(g.stages, g.experts) > kSmemLimit) --g.stages;
+    static bool attr_set[64] = {};
+    const DeviceInfo& dev = device_info();
+    if (!attr_set[dev.index]) {
+        cudaFuncSetAttribute(ragged_pair_kernel<T, MODE, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
+        attr_set[dev.index] = true;
+    }
+    launch_chained(ragged_pair_kernel<T, MODE, RES>, 2 * pairs, kThreads, smem_of(g.stages, g.experts), st, a, b, o, g);
+    count_launch();
+    return launch_status();
+}
+
+// experts, sizes, type, and the offsets' pointer of a call
+int checked(int32_t experts, int64_t T, int32_t N, int32_t K, int dtype) {
+    if (experts < 0 || T < 0 || N < 8 || K < 8 || N % 8 != 0 || K % 8 != 0) return TB200_ERR_SHAPE;
+    if (T > 0x7FFFFE00ll || N > (1 << 28) || K > (1 << 28) || experts > kMaxExperts) return TB200_ERR_SHAPE;
+    if (dtype != TB200_BF16 && dtype != TB200_F16) return TB200_ERR_DTYPE;
+    return TB200_OK;
+}
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+template <typename T>
+int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bool grads, cudaStream_t st) {
+    CUtensorMap ta, tb, to;
+    const uint64_t rows = static_cast<uint64_t>(g.T);
+    const int32_t in = grads ? N : K, out = grads ? K : N;
+    if (!make_map(&ta, x, in, rows, 0, 128) || !make_map(&tb, w, K, N, g.experts, grads ? 64 : 128) || !make_map(&to, g.out, out, rows, 0, 32))
+        return TB200_ERR_DRIVER;
+    g.cols = out;
+    g.depth = in;
+    const int64_t most = (g.T / kTile + g.experts) * ((out + kTile - 1) / kTile);
+    const int pairs = static_cast<int>(most < pairs_here() ? most : pairs_here());
+    if (grads) return launch_pairs<T, kRowGrads, false>(ta, tb, to, g, pairs, st);
+    if (g.residual != nullptr) return launch_pairs<T, kRows, true>(ta, tb, to, g, pairs, st);
+    return launch_pairs<T, kRows, false>(ta, tb, to, g, pairs, st);
+}
+
+// rows from which on a tile can be shared by pairs: below, no expert has 2 kSnap blocks
+constexpr int64_t kShareRows = 2 * kSnap * kBlock;
+
+template <typename T>
+int weights_of(const void* x, const void* dy, RaggedArgs g, cudaStream_t st) {
+    CUtensorMap ta, tb, to;
+    const uint64_t rows = static_cast<uint64_t>(g.T);
+    if (!make_map(&ta, dy, g.n, rows, 0, 64) || !make_map(&tb, x, g.cols, rows, 0, 64) || !make_map(&to, g.out, g.cols, g.n, g.experts, 32))
+        return TB200_ERR_DRIVER;
+    const int pairs = pairs_here();
+    const int code = launch_pairs<T, kWeights, false>(ta, tb, to, g, pairs, st);
+    if (code != TB200_OK || g.partial == nullptr) return code;
+    launch_chained(ragged_join_kernel<T>, dim3(pairs - 1, kTile / 32), 256, (g.experts + 1) * 8, st, g, pairs);
+    count_launch();
+    return launch_status();
+}
+
+int64_t bias_most_pieces(int64_t T, int32_t experts) { return T / kBiasRows + (experts < T ? experts : T); }
+
+}  // namespace
+}  // namespace tb200
+
+extern "C" int tb200_ragged_gemm(const void* x, const void* w, const int32_t* offsets, const float* bias, const void* residual, void* out,
+                                 int32_t experts, int64_t T, int32_t N, int32_t K, int32_t act, int32_t clear, int dtype, int32_t* status_word,
+                                 void* stream) {
+    using namespace tb200;
+    const int code = checked(experts, T, N, K, dtype);
+    if (code != TB200_OK) return code;
+    if (act < 0 || act > 1) return TB200_ERR_UNSUPPORTED;
+    if (T == 0) return TB200_OK;
+    if (x == nullptr || out == nullptr || offsets == nullptr || (experts > 0 && w == nullptr)) return TB200_ERR_NULL;
+    if (!aligned16(x) || !aligned16(w) || !aligned16(out) || !aligned16(residual) || !aligned16(bias) || !aligned4(offsets)) return TB200_ERR_ALIGN;
+    if (!device_info().valid) return TB200_ERR_DEVICE;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (experts == 0) return clear ? static_cast<int>(cudaMemsetAsync(out, 0, static_cast<size_t>(T) * N * 2, st)) : TB200_OK;
+    RaggedArgs g{};
+    g.offsets = offsets;
+    g.bias = bias;
+    g.residual = residual;
+    g.out = out;
+    g.status = status_word;
+    g.experts = experts;
+    g.T = T;
+    g.silu = act;
+    g.clear = clear ? 1 : 0;
+    return dtype == TB200_BF16 ? rows_of<__nv_bfloat16>(x, w, g, N, K, false, st) : rows_of<__half>(x, w, g, N, K, false, st);
+}
+
+extern "C" int tb200_ragged_gemm_dgrad(const void* dy, const void* w, const int32_t* offsets, void* dx, int32_t experts, int64_t T, int32_t N,
+                                       int32_t K, int dtype, int32_t* status_word, void* stream) {
+    using namespace tb200;
+    const int code = checked(experts, T, N, K, dtype);
+    if (code != TB200_OK) return code;
+    if (T == 0) return TB200_OK;
+    if (dy == nullptr || dx == nullptr || offsets == nullptr || (experts > 0 && w == nullptr)) return TB200_ERR_NULL;
+    if (!aligned16(dy) || !aligned16(w) || !aligned16(dx) || !aligned4(offsets)) return TB200_ERR_ALIGN;
+    if (!device_info().valid) return TB200_ERR_DEVICE;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (experts == 0) return static_cast<int>(cudaMemsetAsync(dx, 0, static_cast<size_t>(T) * K * 2, st));
+    RaggedArgs g{};
+    g.offsets = offsets;
+    g.out = dx;
+    g.status = status_word;
+    g.experts = experts;
+    g.T = T;
+    g.clear = 1;
+    return dtype == TB200_BF16 ? rows_of<__nv_bfloat16>(dy, w, g, N, K, true, st) : rows_of<__half>(dy, w, g, N, K, true, st);
+}
+
+extern "C" int64_t tb200_ragged_wgrad_workspace_bytes(int32_t experts, int64_t T, int32_t N, int32_t K) {
+    using namespace tb200;
+    if (checked(experts, T, N, K, TB200_BF16) != TB200_OK || experts == 0) return 0;
+    const int64_t parts = T >= kShareRows ? static_cast<int64_t>(pairs_here()) * 2 * kPartFloats : 0;
+    return 4 * (parts + bias_most_pieces(T, experts) * N);
+}
+
+extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int32_t* offsets, void* dw, float* db, float* workspace, int32_t experts,
+                                       int64_t T, int32_t N, int32_t K, int dtype, int32_t* status_word, void* stream) {
+    using namespace tb200;
+    int code = checked(experts, T, N, K, dtype);
+    if (code != TB200_OK) return code;
+    if (experts == 0) return TB200_OK;
+    if ((dw == nullptr && db == nullptr) || (T > 0 && (dy == nullptr || offsets == nullptr || workspace == nullptr || (x == nullptr && dw != nullptr))))
+        return TB200_ERR_NULL;
+    if (!aligned16(x) || !aligned16(dy) || !aligned16(dw) || !aligned16(workspace) || !aligned4(db) || !aligned4(offsets)) return TB200_ERR_ALIGN;
+    if (!device_info().valid) return TB200_ERR_DEVICE;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (T == 0) {
+        cudaError_t err = cudaSuccess;
+        if (dw != nullptr) err = cudaMemsetAsync(dw, 0, static_cast<size_t>(experts) * N * K * 2, st);
+        if (err == cudaSuccess && db != nullptr) err = cudaMemsetAsync(db, 0, static_cast<size_t>(experts) * N * 4, st);
+        return static_cast<int>(err);
+    }
+    RaggedArgs g{};
+    g.offsets = offsets;
+    g.out = dw;
+    g.status = status_word;
+    g.experts = experts;
+    g.T = T;
+    g.cols = K;
+    g.n = N;
+    g.partial = T >= kShareRows ? workspace : nullptr;
+    if (dw != nullptr) code = dtype == TB200_BF16 ? weights_of<__nv_bfloat16>(x, dy, g, st) : weights_of<__half>(x, dy, g, st);
+    if (code != TB200_OK || db == nullptr) return code;
+    float* part = workspace + (T >= kShareRows ? static_cast<int64_t>(pairs_here()) * 2 * kPartFloats : 0);
+    const int pieces = static_cast<int>(bias_most_pieces(T, experts));
+    const dim3 grid(pieces, (N + 255) / 256);
+    const size_t smem = (static_cast<size_t>(experts) + 1) * 8;
+    if (dtype == TB200_BF16)
+        launch_chained(ragged_bias_part_kernel<__nv_bfloat16>, grid, 256, smem, st, static_cast<const __nv_bfloat16*>(dy), g, part, pieces);
+    else
+        launch_chained(ragged_bias_part_kernel<__half>, grid, 256, smem, st, static_cast<const __half*>(dy), g, part, pieces);
+    launch_chained(ragged_bias_sum_kernel, dim3(experts, (N + 255) / 256), 256, smem, st, g, part, db, pieces);
+    count_launch();
+    count_launch();
+    return launch_status();
+}

@@ -1746,6 +1746,150 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     return out[0] if squeeze else out
 
 
+# --------------------------------------------------------------------------------------------
+# linear layers grouped by expert with ragged sizes
+# --------------------------------------------------------------------------------------------
+def _ragged_operands(name: str, rows: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, width: int):
+    """rows [T, ...], weight [E, N, K], offsets [E + 1]; `width`: the dimension of weight that rows' last dimension has to match."""
+    if rows.ndim != 2 or weight.ndim != 3:
+        raise ValueError(f"{name} needs rows [T, width] and weight [E, N, K]")
+    if rows.shape[1] != weight.shape[width]:
+        raise ValueError(f"{name}: rows of width {rows.shape[1]} do not fit weight {tuple(weight.shape)}")
+    if offsets.ndim != 1 or offsets.shape[0] != weight.shape[0] + 1:
+        raise ValueError(f"{name} offsets must be [E + 1] = [{weight.shape[0] + 1}], got {tuple(offsets.shape)}")
+    if offsets.dtype != torch.int32:
+        raise ValueError(f"{name} offsets must be int32, got {offsets.dtype}")
+    if weight.shape[1] % 8 or weight.shape[2] % 8 or weight.shape[1] < 8 or weight.shape[2] < 8:
+        raise ValueError(f"{name} needs N % 8 == 0 and K % 8 == 0")
+    _require_backend(name, "cuda")
+    _require_cuda_tensors(f"cuda {name}", rows, weight, offsets)
+    if rows.dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError(f"cuda {name} does not support dtype {rows.dtype}")
+    if weight.dtype != rows.dtype:
+        raise ValueError(f"{name} needs rows and weight of one dtype, got {rows.dtype} and {weight.dtype}")
+
+
+def _raise_incomplete(name: str, check: bool, status: torch.Tensor | None) -> None:
+    if check and int(status.item()) != 0:
+        raise RuntimeError(f"cuda {name}: a bounded wait inside the kernel gave up; the output is incomplete")
+
+
+def ragged_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, bias: torch.Tensor | None = None, *, silu: bool = False,
+                  residual: torch.Tensor | None = None, out: torch.Tensor | None = None, checkpoint: bool = False, check: bool = False,
+                  status: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[r] = act(x[r] @ weight[e].T + bias[e]) (+ residual[r])`` for the rows r in [offsets[e], offsets[e + 1]) of every
+    expert e: linear layers grouped by expert, with sizes that only the device knows (tcgen05, fp32 accumulation).
+
+    x: [T, K] with the rows sorted by expert; weight: [E, N, K]; offsets: int32 [E + 1] on the device, not decreasing (one
+    that is counts as the largest before it, and all are held inside [0, T]); bias: [E, N] (any float dtype; used as fp32);
+    residual / out: [T, N]; ``out`` may be ``residual``.  fp16 or bf16; N and K are multiples of 8.  Rows of no expert are
+    zero in a fresh result and left as they are in ``out``.
+
+    Differentiable in x, weight, bias and residual (without ``silu`` and ``out``).  ``checkpoint=True`` keeps x for the
+    weight gradient in 8 bits (``checkpoint_activation``; K a multiple of 128) instead of as it is.  ``check`` / ``status``: as
+    in ``grouped_linear``."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        if silu or out is not None:
+            raise RuntimeError("cuda ragged_linear is forward-only with silu or out: use silu_gate(gated=False) behind it for training")
+        _ragged_operands("ragged_linear", x, weight, offsets, 2)
+        return _RaggedLinearFunction.apply(x, weight, offsets, bias, residual, bool(checkpoint))
+    if _TIMING is None and not check:
+        fast = _host.ragged_linear(x, weight, offsets, bias, silu, residual, out, status)
+        if fast is not None:
+            return fast
+    _ragged_operands("ragged_linear", x, weight, offsets, 2)
+    _require_cuda_tensors("cuda ragged_linear", x, bias, residual, out)
+    rows, k = x.shape
+    experts, n, _k = weight.shape
+    if bias is not None and tuple(bias.shape) != (experts, n):
+        raise ValueError(f"ragged_linear bias must be [E, N] = {(experts, n)}, got {tuple(bias.shape)}")
+    bias32 = None if bias is None else _aligned(bias.to(torch.float32))
+    for what, t in (("residual", residual), ("out", out)):
+        if t is not None and (tuple(t.shape) != (rows, n) or t.dtype != x.dtype):
+            raise ValueError(f"ragged_linear: {what} must be a [T, N] tensor of x's dtype")
+    if out is not None and (not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError("ragged_linear: out must be contiguous and on a 16-byte boundary")
+    x, weight = _aligned(x), _aligned(weight)
+    res = None if residual is None else _aligned(residual)
+    target = torch.empty(rows, n, dtype=x.dtype, device=x.device) if out is None else out
+    status = _status_word(check, status, x.device)
+    with torch.cuda.device(x.device), _timed("ragged_linear", experts=experts, m=rows, n=n, k=k, silu=bool(silu)):
+        code = _lib.load().tb200_ragged_gemm(_ptr(x), _ptr(weight), _ptr(offsets.contiguous()), _ptr(bias32), _ptr(res), _ptr(target), experts, rows,
+                                             n, k, int(bool(silu)), int(out is None), _DTYPE_CODES[x.dtype], _ptr(status), _stream_ptr())
+    _lib.check(code, "cuda ragged_linear")
+    _raise_incomplete("ragged_linear", check, status)
+    return target
+
+
+def ragged_linear_backward(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, grad_out: torch.Tensor, *,
+                           scales: torch.Tensor | None = None, bias: bool = False, need_x: bool = True, need_weight: bool = True,
+                           check: bool = False, status: torch.Tensor | None = None
+                           ) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """(dx, dweight, dbias) of ``ragged_linear(x, weight, offsets, bias)``: ``dx[r] = grad_out[r] @ weight[e]``,
+    ``dweight[e] = grad_out_e.T @ x_e`` in weight's dtype, ``dbias[e]`` (with ``bias=True``) the fp32 sum of the expert's rows.
+
+    With ``scales`` x is the e4m3 half of a ``checkpoint_activation`` pair.  Rows of no expert get a zero ``dx`` and take no part in
+    the sums; an expert without rows gets zeros.  What is not needed comes back as None.  The sums run in a fixed order."""
+    if _TIMING is None and not check and scales is None and need_x and need_weight:
+        fast = _host.ragged_linear_backward(x, weight, offsets, grad_out, bias, status)
+        if fast is not None:
+            return fast
+    if x.ndim != 2 or grad_out.ndim != 2 or grad_out.shape[0] != x.shape[0]:
+        raise ValueError("ragged_linear_backward needs x [T, K] and grad_out [T, N]")
+    _ragged_operands("ragged_linear_backward", grad_out, weight, offsets, 1)
+    if x.shape[1] != weight.shape[2]:
+        raise ValueError(f"ragged_linear_backward: x of width {x.shape[1]} does not fit weight {tuple(weight.shape)}")
+    _require_cuda_tensors("cuda ragged_linear_backward", x, grad_out, scales)
+    if scales is None and x.dtype != grad_out.dtype:
+        raise ValueError(f"ragged_linear_backward needs x and grad_out of one dtype, got {x.dtype} and {grad_out.dtype}")
+    rows, k = x.shape
+    experts, n, _k = weight.shape
+    dev = x.device
+    dy, w, off = _aligned(grad_out.detach()), _aligned(weight.detach()), offsets.contiguous()
+    lib, dt = _lib.load(), _DTYPE_CODES[dy.dtype]
+    status = _status_word(check, status, dev)
+    dx = dw = db = None
+    with torch.cuda.device(dev):
+        if need_x:
+            dx = torch.empty(rows, k, dtype=dy.dtype, device=dev)
+            with _timed("ragged_linear_dgrad", experts=experts, m=rows, n=k, k=n):
+                code = lib.tb200_ragged_gemm_dgrad(_ptr(dy), _ptr(w), _ptr(off), _ptr(dx), experts, rows, n, k, dt, _ptr(status), _stream_ptr())
+            _lib.check(code, "cuda ragged_linear_backward")
+        if need_weight or bias:
+            kept = None if not need_weight else _aligned(x.detach()) if scales is None else restore_activation(x, scales, dy.dtype)
+            dw = torch.empty(experts, n, k, dtype=dy.dtype, device=dev) if need_weight else None
+            db = torch.empty(experts, n, dtype=torch.float32, device=dev) if bias else None
+            work = torch.empty(max(int(lib.tb200_ragged_wgrad_workspace_bytes(experts, rows, n, k)) // 4, 1), dtype=torch.float32, device=dev)
+            with _timed("ragged_linear_wgrad", experts=experts, m=n, n=k, k=rows):
+                code = lib.tb200_ragged_gemm_wgrad(_ptr(kept), _ptr(dy), _ptr(off), _ptr(dw), _ptr(db), _ptr(work), experts, rows, n, k, dt,
+                                                   _ptr(status), _stream_ptr())
+            _lib.check(code, "cuda ragged_linear_backward")
+    _raise_incomplete("ragged_linear_backward", check, status)
+    return dx, dw, db
+
+
+class _RaggedLinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets, bias, residual, checkpoint):
+        kept = scales = None
+        if weight.requires_grad:
+            kept, scales = checkpoint_activation(x) if checkpoint else (x, None)
+        ctx.save_for_backward(kept, scales, weight, offsets)
+        ctx.rows = x.shape
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        with torch.no_grad():
+            return ragged_linear(x, weight, offsets, bias, residual=residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        kept, scales, weight, offsets = ctx.saved_tensors
+        need_x, need_w, _o, need_b, need_r, _c = ctx.needs_input_grad
+        x = kept if kept is not None else grad_out.new_empty(1).expand(ctx.rows)     # its shape alone is read
+        dx, dw, db = ragged_linear_backward(x, weight, offsets, grad_out, scales=scales, bias=need_b, need_x=need_x, need_weight=need_w)
+        return dx, dw, None, None if db is None else db.to(ctx.bias_dtype), grad_out if need_r else None, None
+
+
 def ffn_fp8_static_capacity() -> int:
     """Bytes of the fixed in-library scratch array used by ``ffn_fp8_static`` (per GPU)."""
     return int(_lib.load().tb200_ffn_fp8_static_scratch_bytes())
@@ -2316,4 +2460,14 @@ __all__ = [
     "scatter_rows",
     "sequence_gather",
     "sequence_prepare",
+    "add_rms_norm",
+    "add_rms_norm_backward",
+    "add_rms_norm_quant",
+    "checkpoint_activation",
+    "restore_activation",
+    "silu_gate",
+    "silu_gate_backward",
+    "silu_gate_checkpoint",
+    "ragged_linear",
+    "ragged_linear_backward",
 ]

@@ -100,3 +100,53 @@ def test_kept_activation_entries(lib):
     assert fwd(P(p), P(p + 8), None, None, 4, 128, 1, 1, BF16, None) == ERR_ALIGN
     assert bwd(P(p), P(p), None, P(p), None, 4, 128, 1, 1, BF16, None) == ERR_NULL
     assert bwd(P(p), P(p), P(p), P(p), P(p + 8), 4, 128, 1, 1, BF16, None) == ERR_ALIGN
+
+
+def test_ragged_shapes_are_looked_at_first():
+    x, w, off = torch.ones(6, 64), torch.ones(2, 16, 64), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="rows \\[T, width\\]"):
+        ops.ragged_linear(x[None], w, off)
+    with pytest.raises(ValueError, match="do not fit weight"):
+        ops.ragged_linear(x[:, :32], w, off)
+    with pytest.raises(ValueError, match="offsets must be \\[E \\+ 1\\]"):
+        ops.ragged_linear(x, w, off[:2])
+    with pytest.raises(ValueError, match="offsets must be int32"):
+        ops.ragged_linear(x, w, off.long())
+    with pytest.raises(ValueError, match="N % 8"):
+        ops.ragged_linear(x, w[:, :12], off)
+    with pytest.raises(ValueError, match="grad_out"):
+        ops.ragged_linear_backward(x, w, off, torch.ones(5, 16))
+    with pytest.raises(ValueError, match="do not fit weight"):
+        ops.ragged_linear_backward(x, w, off, torch.ones(6, 24))
+
+
+def test_ragged_has_no_cpu_path(monkeypatch):
+    monkeypatch.setattr(ops, "cuda_available", lambda: True)
+    x, w, off = torch.ones(6, 64).bfloat16(), torch.ones(2, 16, 64).bfloat16(), torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: ops.ragged_linear(x, w, off), lambda: ops.ragged_linear_backward(x, w, off, x[:, :16].contiguous())):
+        with pytest.raises(RuntimeError, match="requires CUDA tensors"):
+            call()
+
+
+def test_ragged_entries(lib):
+    buf = (ctypes.c_uint8 * 256)()
+    p = (ctypes.addressof(buf) + 15) & ~15
+
+    def rows(x=P(p), w=P(p), off=P(p), bias=None, res=None, out=P(p), experts=2, T=4, n=64, k=64, act=0, dtype=BF16):
+        return lib.tb200_ragged_gemm(x, w, off, bias, res, out, experts, T, n, k, act, 1, dtype, None, None)
+
+    assert rows(T=0) == OK
+    assert rows(T=-1) == ERR_SHAPE and rows(n=12) == ERR_SHAPE and rows(k=0) == ERR_SHAPE and rows(experts=5000) == ERR_SHAPE
+    assert rows(T=1 << 31) == ERR_SHAPE                                    # row numbers are held in 32 bits
+    assert rows(dtype=0) == ERR_DTYPE and rows(act=2) == ERR_UNSUPPORTED
+    assert rows(x=None) == ERR_NULL and rows(off=None) == ERR_NULL and rows(w=None) == ERR_NULL and rows(out=None) == ERR_NULL
+    assert rows(x=P(p + 2)) == ERR_ALIGN and rows(res=P(p + 8)) == ERR_ALIGN and rows(bias=P(p + 4)) == ERR_ALIGN and rows(off=P(p + 2)) == ERR_ALIGN
+    dgrad, wgrad = lib.tb200_ragged_gemm_dgrad, lib.tb200_ragged_gemm_wgrad
+    assert dgrad(P(p), P(p), P(p), P(p), 2, 0, 64, 64, BF16, None, None) == OK
+    assert dgrad(P(p), None, P(p), P(p), 2, 4, 64, 64, BF16, None, None) == ERR_NULL
+    assert dgrad(P(p), P(p), P(p), P(p + 8), 2, 4, 64, 64, BF16, None, None) == ERR_ALIGN
+    assert wgrad(P(p), P(p), P(p), P(p), None, P(p), 0, 4, 64, 64, BF16, None, None) == OK
+    assert wgrad(P(p), P(p), P(p), None, None, P(p), 2, 4, 64, 64, BF16, None, None) == ERR_NULL
+    assert wgrad(P(p), P(p), P(p), P(p), None, None, 2, 4, 64, 64, BF16, None, None) == ERR_NULL
+    assert wgrad(None, P(p), P(p), P(p), None, P(p), 2, 4, 64, 64, BF16, None, None) == ERR_NULL
+    assert wgrad(P(p), P(p), P(p), P(p), P(p + 2), P(p), 2, 4, 64, 64, BF16, None, None) == ERR_ALIGN
