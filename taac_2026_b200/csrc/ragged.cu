@@ -18,11 +18,9 @@
 //              the MMAs see them.
 // A row tile that crosses its expert's end computes rows of the next expert for nothing and does not store them.
 //
-// Distribution.  Row tiles go round robin over the pairs.  The weight gradient of uneven experts does not: its tiles
-// differ in length, so all tiles' 64-row blocks are lined up and every pair takes an equal share of the line; a tile that
-// two or more pairs share leaves fp32 partial tiles in a workspace, which `ragged_join_kernel` adds in the order of the
-// pairs.  Shares that would leave less than kSnap blocks of a tile move to the tile's edge: writing and reading a partial tile costs
-// about as much as that many blocks.
+// Distribution.  Row tiles go round robin over the pairs.  The tiles of the weight gradients of uneven experts differ in
+// length: most go round robin as well, the rest is cut into shares that even the pairs out (see Line), and a tile that two or
+// more pairs share leaves fp32 partial tiles in a workspace, which `ragged_join_kernel` adds in the order of the pairs.
 //
 // Every wait on an mbarrier is bounded; a wait that gives up raises the status word and all roles drain through the final barrier.
 #include "tb200_common.cuh"
@@ -46,8 +44,8 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + kEpiWarps * 32;
 constexpr uint32_t kBoxBytes = 32 * 128;                  // an epilogue warp's staging box: 32 rows x 64 columns
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMaxExperts = 4096;
-constexpr int kSnap = 8;
+constexpr int kMaxExperts = 2048;
+constexpr int kSnap = 4;
 constexpr int64_t kPartFloats = int64_t(kTile) * kTile;   // of a partial tile
 constexpr size_t kSmemLimit = 227 * 1024 - 512;           // less the static part
 
@@ -57,6 +55,7 @@ struct RaggedArgs {
     const void* residual;       // [T, cols] or NULL (rows)
     void* out;                  // [T, cols], or [experts, n, k] (weights)
     float* partial;             // [pairs][2] partial tiles, NULL: tiles are never shared (weights)
+    int4* pieces;               // [pairs][2] what they are part of: expert (-1: nothing), first row and column of the tile, last piece?
     int32_t* status;
     int32_t experts, stages;
     int64_t T;
@@ -67,29 +66,9 @@ struct RaggedArgs {
     int32_t clear;              // rows of no expert are set to zero
 };
 
-// Units of work of `rows` rows: row tiles, 64-row blocks (an expert without rows has one: the zeros of its weight gradient are
-// written), or the pieces of the bias gradient
-enum Units : int { kTiles, kBlocks, kBiasPieces };
-constexpr int kBiasRows = 256;
-template <int U>
-__device__ __forceinline__ int units_of(int rows) {
-    if (U == kTiles) return (rows + kTile - 1) / kTile;
-    if (U == kBlocks) return rows == 0 ? 1 : (rows + kBlock - 1) / kBlock;
-    return (rows + kBiasRows - 1) / kBiasRows;
-}
-// Where every expert's rows begin, and how many units the experts before it have.  An offset outside [0, T] is moved to
+// Where every expert's rows begin, by one warp; the offsets come from the kernel in front.  An offset outside [0, T] is moved to
 // the nearer end and one that lies before an earlier one counts as that one, so that no two experts share a row.
-struct Plan {
-    int32_t* begin;    // [experts + 1] in shared memory
-    int32_t* pre;      // [experts + 1]
-};
-__device__ __forceinline__ Plan plan_at(void* smem, int experts) {
-    int32_t* p = static_cast<int32_t*>(smem);
-    return Plan{p, p + experts + 1};
-}
-// By one warp; the offsets come from the kernel in front.
-template <int U>
-__device__ void make_plan(const RaggedArgs& g, const Plan& plan, int lane) {
+__device__ void first_rows(const RaggedArgs& g, int32_t* begin, int lane) {
     int32_t top = 0;
     for (int base = 0; base <= g.experts; base += 32) {
         int32_t v = 0;
@@ -101,25 +80,29 @@ __device__ void make_plan(const RaggedArgs& g, const Plan& plan, int lane) {
             if (lane >= o) v = max(v, u);
         }
         v = max(v, top);
-        if (base + lane <= g.experts) plan.begin[base + lane] = v;
+        if (base + lane <= g.experts) begin[base + lane] = v;
         top = __shfl_sync(0xffffffffu, v, 31);
     }
     __syncwarp();
+}
+// pre[i] = sum of units(0 .. i - 1), by one warp
+template <typename F>
+__device__ void prefix(int32_t* pre, int n, int lane, F units) {
     int32_t sum = 0;
-    for (int base = 0; base < g.experts; base += 32) {
-        const int e = base + lane;
-        int32_t v = e < g.experts ? units_of<U>(plan.begin[e + 1] - plan.begin[e]) : 0;
+    for (int base = 0; base < n; base += 32) {
+        int32_t v = base + lane < n ? units(base + lane) : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
-        if (e < g.experts) plan.pre[e + 1] = sum + v;
+        if (base + lane < n) pre[base + lane + 1] = sum + v;
         sum += __shfl_sync(0xffffffffu, v, 31);
     }
-    if (lane == 0) plan.pre[0] = 0;
+    if (lane == 0) pre[0] = 0;
+    __syncwarp();
 }
-// the expert whose units hold `unit`
+// the last i with pre[i] <= unit: the expert whose units hold `unit`
 __device__ __forceinline__ int expert_of(const int32_t* pre, int experts, int64_t unit) {
     int lo = 0, hi = experts;
     while (hi - lo > 1) {
@@ -129,18 +112,102 @@ __device__ __forceinline__ int expert_of(const int32_t* pre, int experts, int64_
     }
     return lo;
 }
-// Begin of pair i's share of the line of blocks, moved to the edge of its tile where it lies near one
-__device__ __forceinline__ int64_t share_begin(const int32_t* pre, int experts, int tiles, int i, int pairs, bool split) {
-    const int64_t total = static_cast<int64_t>(pre[experts]) * tiles;
-    if (i >= pairs) return total;
-    const int64_t p = total / pairs * i + total % pairs * i / pairs;
-    const int e = expert_of(pre, experts, p / tiles);
-    const int64_t base = static_cast<int64_t>(pre[e]) * tiles;
-    const int64_t nb = pre[e + 1] - pre[e];
-    if (nb == 0) return p;
-    const int64_t o = (p - base) % nb, begin = p - o;
-    if (!split) return 2 * o < nb ? begin : begin + nb;
-    return o < kSnap ? begin : (nb - o < kSnap ? begin + nb : p);
+__device__ __forceinline__ int row_tiles(const int32_t* begin, int e) { return (begin[e + 1] - begin[e] + kTile - 1) / kTile; }
+// 64-row blocks of an expert's weight gradient; one without rows has one: its zeros are written
+__device__ __forceinline__ int row_blocks(const int32_t* begin, int e) {
+    const int rows = begin[e + 1] - begin[e];
+    return rows == 0 ? 1 : (rows + kBlock - 1) / kBlock;
+}
+
+// How the tiles of the weight gradients are shared out.  All experts have `tiles` tiles, each as long as its expert has blocks.  The
+// experts stand in a line, those whose tiles are no longer than a pair's equal share in front, and their tiles one after
+// the other.  The first `wave_tiles` of the line go round robin, so that the pairs are on the same few experts at a time and read the
+// same rows while these are in the L2; every pair stays within its equal share there.  What lies behind is cut so that
+// all pairs end up with equal shares.
+struct Line {
+    int32_t* begin;       // [experts + 1] first rows
+    int32_t* pre;         // [experts + 1] blocks of one column of tiles before the i-th expert of the line
+    int32_t* order;       // [experts] expert numbers in the order of the line
+    int64_t* wave_tiles;  // [1]
+    int64_t* cut;         // [2] begin and end of this pair's share of the rest
+};
+__host__ __device__ __forceinline__ size_t line_bytes(int experts) { return 24 + 4 * (3 * static_cast<size_t>(experts) + 2); }
+__device__ __forceinline__ Line line_at(void* smem, int experts) {
+    int64_t* w = static_cast<int64_t*>(smem);
+    int32_t* p = reinterpret_cast<int32_t*>(w + 3);
+    return Line{p, p + experts + 1, p + 2 * (experts + 1), w, w + 1};
+}
+// `p` moved to an edge of its tile where it lies near one: a partial tile costs about as much as kSnap blocks
+__device__ __forceinline__ int64_t snapped(const Line& line, int experts, int tiles, int64_t p) {
+    if (p >= static_cast<int64_t>(line.pre[experts]) * tiles) return p;
+    const int i = expert_of(line.pre, experts, p / tiles);
+    const int64_t nb = line.pre[i + 1] - line.pre[i], o = (p - static_cast<int64_t>(line.pre[i]) * tiles) % nb;
+    return o < kSnap ? p - o : (nb - o < kSnap ? p - o + nb : p);
+}
+// By one warp, for one of the pairs.
+__device__ void make_line(const RaggedArgs& g, const Line& line, int tiles, int pairs, int pair, int lane) {
+    first_rows(g, line.begin, lane);
+    if (g.partial == nullptr) {      // no tile is ever shared: all of them go round robin
+        prefix(line.pre, g.experts, lane, [&](int e) { return row_blocks(line.begin, e); });
+        for (int e = lane; e < g.experts; e += 32) line.order[e] = e;
+        if (lane == 0) {
+            *line.wave_tiles = static_cast<int64_t>(g.experts) * tiles;
+            line.cut[0] = line.cut[1] = 0;
+        }
+        __syncwarp();
+        return;
+    }
+    int32_t sum = 0;
+    for (int e = lane; e < g.experts; e += 32) sum += row_blocks(line.begin, e);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int64_t total = static_cast<int64_t>(sum) * tiles, share = total / pairs;
+    int placed = 0, shorter = 0, longest = 1;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int base = 0; base < g.experts; base += 32) {
+            const int e = base + lane;
+            const int nb = e < g.experts ? row_blocks(line.begin, e) : 0;
+            const bool mine = e < g.experts && (nb <= share) == (pass == 0);
+            const uint32_t mask = __ballot_sync(0xffffffffu, mine);
+            if (mine) line.order[placed + __popc(mask & ((1u << lane) - 1))] = e;
+            if (mine && pass == 0) longest = max(longest, nb);
+            placed += __popc(mask);
+        }
+        if (pass == 0) shorter = placed;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+    __syncwarp();
+    prefix(line.pre, g.experts, lane, [&](int i) { return row_blocks(line.begin, line.order[i]); });
+    const int64_t fit = static_cast<int64_t>(shorter) * tiles / pairs;
+    const int64_t waves = fit < share / longest ? fit : share / longest;
+    if (lane == 0) *line.wave_tiles = waves * pairs;
+    int64_t before = 0;      // blocks of the waves that go to the pairs in front
+    const int64_t rest = waves * pairs / tiles;      // the expert that the line's rest begins in
+    const int64_t start = waves * pairs >= static_cast<int64_t>(g.experts) * tiles
+                              ? total : static_cast<int64_t>(line.pre[rest]) * tiles + waves * pairs % tiles * (line.pre[rest + 1] - line.pre[rest]);
+    for (int base = 0; base <= pairs; base += 32) {
+        const int q = base + lane;
+        int64_t load = 0;
+        if (q < pairs) {
+            for (int64_t w = 0; w < waves; ++w) {
+                const int i = static_cast<int>((w * pairs + q) / tiles);
+                load += line.pre[i + 1] - line.pre[i];
+            }
+        }
+        int64_t upto = load;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += u;
+        }
+        if (q == pair || q == pair + 1) {
+            const int64_t p = q == pairs ? total : start + total / pairs * q + total % pairs * q / pairs - (before + upto - load);
+            line.cut[q - pair] = snapped(line, g.experts, tiles, p);
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    __syncwarp();
 }
 
 // One piece of a pair's work
@@ -150,60 +217,76 @@ struct Job {
     int64_t m0;                // rows: first row of the tile; weights: first row of the expert that is contracted
     int32_t a0, b0;            // weights: first dw row and column; rows: b0 = first column of the tile
     int blocks;                // stages of this piece
-    int slot;                  // weights: partial tile that receives it, -1: the whole tile
+    int slot;                  // weights: partial tile that receives it (0: the tile's begin is another pair's), -1: the whole tile
+    bool last;                 // weights: the piece reaches the tile's end
 };
 
+// The pieces of a pair's work, in the order in which every role of the pair walks them
 template <int MODE>
 struct Walk {
     const RaggedArgs& g;
-    const int32_t *first_row, *pre;
+    const Line& line;
     int n_tiles, b_tiles;
-    int64_t at, stop, step;
-    int e = -1;
-    int64_t begin = 0, end = 0;
+    int64_t at, stop, step, wave_stop;
+    int i = -1;                    // place of the expert in the line (rows: its number)
 
-    __device__ Walk(const RaggedArgs& args, const Plan& plan, int pair, int pairs) : g(args), first_row(plan.begin), pre(plan.pre) {
+    __device__ Walk(const RaggedArgs& args, const Line& l, int pair, int pairs) : g(args), line(l) {
         b_tiles = (g.cols + kTile - 1) / kTile;
         n_tiles = MODE == kWeights ? (g.n + kTile - 1) / kTile : 1;
+        at = pair;
+        step = pairs;
         if (MODE == kWeights) {
-            at = share_begin(pre, g.experts, n_tiles * b_tiles, pair, pairs, g.partial != nullptr);
-            stop = share_begin(pre, g.experts, n_tiles * b_tiles, pair + 1, pairs, g.partial != nullptr);
-            step = 0;
+            wave_stop = *line.wave_tiles;
+            stop = line.cut[1];
+            if (at >= wave_stop) rest();
         } else {
-            at = pair;
-            stop = static_cast<int64_t>(pre[g.experts]) * b_tiles;
-            step = pairs;
+            stop = static_cast<int64_t>(line.pre[g.experts]) * b_tiles;
         }
     }
+    __device__ void rest() {       // behind the tiles that go round robin
+        at = line.cut[0];
+        step = 0;
+    }
     __device__ bool next(Job& j) {
-        if (at >= stop) return false;
-        const int per = n_tiles * b_tiles;
-        const int64_t unit = at / per;
-        if (e < 0 || unit >= pre[e + 1]) {
-            e = e < 0 ? expert_of(pre, g.experts, unit) : e + 1;
-            while (unit >= pre[e + 1]) ++e;
-            begin = first_row[e];
-            end = first_row[e + 1];
-        }
-        j.e = e;
-        j.begin = begin;
-        j.end = end;
         if (MODE == kWeights) {
-            const int nb = pre[e + 1] - pre[e];
-            const int64_t local = at - static_cast<int64_t>(pre[e]) * per;
-            const int tile = static_cast<int>(local / nb), first = static_cast<int>(local % nb);
-            const int64_t left = stop - at;
-            const int take = left < nb - first ? static_cast<int>(left) : nb - first;
+            if (step == 0 && at >= stop) return false;
+            const int tiles = n_tiles * b_tiles;
+            int tile, first = 0, nb, take;
+            if (step != 0) {
+                i = static_cast<int>(at / tiles);
+                tile = static_cast<int>(at % tiles);
+                nb = take = line.pre[i + 1] - line.pre[i];
+                at += step;
+                if (at >= wave_stop) rest();
+            } else {
+                i = expert_of(line.pre, g.experts, at / tiles);
+                nb = line.pre[i + 1] - line.pre[i];
+                const int64_t local = at - static_cast<int64_t>(line.pre[i]) * tiles;
+                tile = static_cast<int>(local / nb);
+                first = static_cast<int>(local % nb);
+                take = stop - at < nb - first ? static_cast<int>(stop - at) : nb - first;
+                at += take;
+            }
+            j.e = line.order[i];
+            j.begin = line.begin[j.e];
+            j.end = line.begin[j.e + 1];
             j.a0 = tile / b_tiles * kTile;
             j.b0 = tile % b_tiles * kTile;
-            j.m0 = begin + static_cast<int64_t>(first) * kBlock;
-            j.blocks = end > begin ? take : 0;
+            j.m0 = j.begin + static_cast<int64_t>(first) * kBlock;
+            j.blocks = j.end > j.begin ? take : 0;
             j.slot = take == nb ? -1 : (first > 0 ? 0 : 1);
-            at += take;
+            j.last = first + take == nb;
         } else {
+            if (at >= stop) return false;
+            const int64_t unit = at / b_tiles;
+            if (i < 0) i = expert_of(line.pre, g.experts, unit);
+            while (unit >= line.pre[i + 1]) ++i;
+            j.e = i;
+            j.begin = line.begin[i];
+            j.end = line.begin[i + 1];
             j.b0 = static_cast<int>(at % b_tiles) * kTile;
             j.a0 = 0;
-            j.m0 = begin + (unit - pre[e]) * kTile;
+            j.m0 = j.begin + (unit - line.pre[i]) * kTile;
             j.blocks = (g.depth + kBlock - 1) / kBlock;
             j.slot = -1;
             at += step;
@@ -241,7 +324,7 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
 
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* out_s = ring + static_cast<size_t>(g.stages) * kStageBytes;
-    const Plan plan = plan_at(out_s + kEpiWarps * kBoxBytes, g.experts);
+    const Line line = line_at(out_s + kEpiWarps * kBoxBytes, g.experts);
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();         // 0 = leader
@@ -270,10 +353,17 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     const uint32_t tmem_base = tmem_base_slot;
     chain_release();                              // not before every CTA holds its tensor memory (see launch_chained)
     chain_wait();
-    if (warp == 0) make_plan<MODE == kWeights ? kBlocks : kTiles>(g, plan, lane);
+    if (warp == 0) {
+        if (MODE == kWeights) {
+            make_line(g, line, (g.n + kTile - 1) / kTile * ((g.cols + kTile - 1) / kTile), pairs, pair, lane);
+        } else {
+            first_rows(g, line.begin, lane);
+            prefix(line.pre, g.experts, lane, [&](int e) { return row_tiles(line.begin, e); });
+        }
+    }
     __syncthreads();
 
-    Walk<MODE> walk(g, plan, pair, pairs);
+    Walk<MODE> walk(g, line, pair, pairs);
     Job j;
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer (both CTAs)
@@ -421,7 +511,7 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         const int swz = lane & 7;
         T* out = static_cast<T*>(g.out);
         if (MODE != kWeights && g.clear) {        // rows in front of the first expert and behind the last
-            const int64_t head = plan.begin[0], owned = plan.begin[g.experts] - head;
+            const int64_t head = line.begin[0], owned = line.begin[g.experts] - head;
             const int64_t row_pieces = g.cols / 8, pieces = (g.T - owned) * row_pieces;
             for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kEpiWarps * 32) + threadIdx.x - 64; i < pieces;
                  i += static_cast<int64_t>(gridDim.x) * (kEpiWarps * 32)) {
@@ -433,6 +523,7 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         }
         uint32_t buf = 0, aph = 0;
         bool ok = true;
+        int4 left0 = make_int4(-1, 0, 0, 0), left1 = left0;
         while (walk.next(j)) {
             const bool none = MODE == kWeights && j.blocks == 0;      // zeros, without the tensor cores
             const int64_t row0 = MODE == kWeights ? j.a0 + static_cast<int>(rank) * 128 + quarter * 32
@@ -442,12 +533,24 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             const bool boxed = MODE == kWeights || row0 + 32 <= row_end;
             const bool live = row < row_end;
             const int col0 = j.b0 + half * 128;
-            const float* bias_t = MODE == kRows && g.bias != nullptr ? g.bias + static_cast<int64_t>(j.e) * g.cols : nullptr;
+            // the bias of a piece is asked for a piece ahead (behind the tile's last column: of its last columns, not used)
+            const bool biased = MODE == kRows && g.bias != nullptr;
+            const float* bias_t = biased ? g.bias + static_cast<int64_t>(j.e) * g.cols : nullptr;
+            float4 bias[MODE == kRows ? 8 : 1];
+            auto fetch_bias = [&](int col) {
+                if (biased) {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) bias[MODE == kRows ? q : 0] = __ldg(reinterpret_cast<const float4*>(bias_t + min(col + 4 * q, g.cols - 4)));
+                }
+            };
+            fetch_bias(col0);
             const T* res_row = RES ? static_cast<const T*>(g.residual) + row * g.cols : nullptr;
             float* part = nullptr;
-            if (MODE == kWeights && j.slot >= 0)
+            if (MODE == kWeights && j.slot >= 0) {
+                (j.slot == 0 ? left0 : left1) = make_int4(j.e, j.a0, j.b0, j.last);
                 part = g.partial + (static_cast<int64_t>(pair) * 2 + j.slot) * kPartFloats + static_cast<int64_t>(rank) * (kPartFloats / 2) +
                        (quarter * 32 + lane) * 4;
+            }
             // A warp whose wait gives up stops waiting but keeps walking (it still arrives on the accumulator barrier).
             if (ok && !none) {
                 int passed = 1;
@@ -495,8 +598,8 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(acc[8 * q + e]);
                     if (MODE == kRows) {
-                        if (bias_t != nullptr && c < g.cols) {
-                            const float4 b0 = __ldg(reinterpret_cast<const float4*>(bias_t + c)), b1 = __ldg(reinterpret_cast<const float4*>(bias_t + c + 4));
+                        if (biased) {
+                            const float4 b0 = bias[MODE == kRows ? 2 * q : 0], b1 = bias[MODE == kRows ? 2 * q + 1 : 0];
                             v[0] += b0.x; v[1] += b0.y; v[2] += b0.z; v[3] += b0.w;
                             v[4] += b1.x; v[5] += b1.y; v[6] += b1.z; v[7] += b1.w;
                         }
@@ -515,6 +618,7 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                     if (boxed) *reinterpret_cast<uint4*>(box + lane * 128 + (((sub * 4 + q) ^ swz) << 4)) = w;
                     else if (live && c < g.cols) *reinterpret_cast<uint4*>(out + row * g.cols + c) = w;
                 }
+                if (piece < 3) fetch_bias(col + 32);
                 if (sub == 1 && boxed) {
                     fence_proxy_async_smem();
                     __syncwarp();
@@ -530,6 +634,10 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                 aph ^= buf;
                 buf ^= 1;
             }
+        }
+        if (MODE == kWeights && g.partial != nullptr && rank == 0 && ew == 0 && lane == 0) {
+            g.pieces[2 * pair] = left0;
+            g.pieces[2 * pair + 1] = left1;
         }
         if (lane == 0) bulk_wait<0>();            // the last store must have left shared memory before the CTA ends
         if (!ok) {
@@ -547,29 +655,16 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     }
 }
 
-// Adds the partial tiles of every shared weight-gradient tile.  CTA x of column y looks at the border between the shares of pairs x and
-// x + 1: if it lies inside a tile and is the first to do so, the CTA adds what the pairs left there, in their order, for 32 of
-// the tile's columns (a thread holds one of the 256 rows).
+// Adds the partial tiles of every shared weight-gradient tile.  CTA (x, y): if pair x left the begin of a tile, what the pairs behind it
+// left of the same tile is added to it, in their order, for 32 of the tile's columns (a thread holds one of the 256 rows).
 template <typename T>
 __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, int pairs) {
-    extern __shared__ int32_t plan_s[];
-    const Plan plan = plan_at(plan_s, g.experts);
-    const int32_t* pre = plan.pre;
     chain_release();
     chain_wait();
-    if (threadIdx.x < 32) make_plan<kBlocks>(g, plan, threadIdx.x);
-    __syncthreads();
-    const int b_tiles = (g.cols + kTile - 1) / kTile, tiles = (g.n + kTile - 1) / kTile * b_tiles;
-    const int i = blockIdx.x + 1;
-    const int64_t p = share_begin(pre, g.experts, tiles, i, pairs, true), total = static_cast<int64_t>(pre[g.experts]) * tiles;
-    if (p >= total) return;
-    const int e = expert_of(pre, g.experts, p / tiles);
-    const int64_t base = static_cast<int64_t>(pre[e]) * tiles, nb = pre[e + 1] - pre[e];
-    const int64_t begin = p - (p - base) % nb, end = begin + nb;
-    if (p == begin || share_begin(pre, g.experts, tiles, i - 1, pairs, true) > begin) return;
-    const int tile = static_cast<int>((begin - base) / nb);
+    const int4 mine = __ldcg(g.pieces + 2 * blockIdx.x + 1);
+    if (mine.x < 0) return;
     const int r = threadIdx.x;
-    const int row = tile / b_tiles * kTile + r, col = tile % b_tiles * kTile + blockIdx.y * 32;
+    const int row = mine.y + r, col = mine.z + blockIdx.y * 32;
     float4 sum[8];
     auto add = [&](int pair, int slot, bool first) {
         const float* part = g.partial + (static_cast<int64_t>(pair) * 2 + slot) * kPartFloats + (r >> 7) * (kPartFloats / 2) + (r & 127) * 4;
@@ -580,15 +675,15 @@ __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, in
             else sum[q] = make_float4(sum[q].x + v.x, sum[q].y + v.y, sum[q].z + v.z, sum[q].w + v.w);
         }
     };
-    add(i - 1, 1, true);
-    int64_t lo = p;
-    for (int k = i; k < pairs && lo < end; ++k) {
-        const int64_t hi = share_begin(pre, g.experts, tiles, k + 1, pairs, true);
-        if (hi > lo) add(k, 0, false);
-        lo = hi;
+    add(blockIdx.x, 1, true);
+    for (int k = blockIdx.x + 1; k < pairs; ++k) {
+        const int4 next = __ldcg(g.pieces + 2 * k);
+        if (next.x < 0) continue;      // a pair without a share
+        add(k, 0, false);
+        if (next.w != 0) break;
     }
     if (row >= g.n) return;
-    T* out = static_cast<T*>(g.out) + (static_cast<int64_t>(e) * g.n + row) * g.cols;
+    T* out = static_cast<T*>(g.out) + (static_cast<int64_t>(mine.x) * g.n + row) * g.cols;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         if (col + q * 8 >= g.cols) break;
@@ -600,21 +695,26 @@ __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, in
 
 // db[e] = sum of the expert's rows of dy, in two steps of fixed order.  Step one: CTA (x, y) adds up to kBiasRows rows (a piece of
 // one expert) for 256 columns; its eight warps take every eighth row, eight columns a lane.
+constexpr int kBiasRows = 256;
+__device__ void bias_pieces(const RaggedArgs& g, int32_t* begin, int32_t* pre, int lane) {
+    first_rows(g, begin, lane);
+    prefix(pre, g.experts, lane, [&](int e) { return (begin[e + 1] - begin[e] + kBiasRows - 1) / kBiasRows; });
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) ragged_bias_part_kernel(const T* __restrict__ dy, const RaggedArgs g, float* __restrict__ part, int max_pieces) {
-    extern __shared__ int32_t plan_s[];
+    extern __shared__ int32_t begin[];
     __shared__ float sums[8][256];
-    const Plan plan = plan_at(plan_s, g.experts);
-    const int32_t* pre = plan.pre;
+    int32_t* pre = begin + g.experts + 1;
     chain_release();
     chain_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) make_plan<kBiasPieces>(g, plan, lane);
+    if (warp == 0) bias_pieces(g, begin, pre, lane);
     __syncthreads();
     const int piece = blockIdx.x;
     if (piece >= pre[g.experts] || piece >= max_pieces) return;
     const int e = expert_of(pre, g.experts, piece);
-    const int64_t first = plan.begin[e] + static_cast<int64_t>(piece - pre[e]) * kBiasRows, end = plan.begin[e + 1];
+    const int64_t first = begin[e] + static_cast<int64_t>(piece - pre[e]) * kBiasRows, end = begin[e + 1];
     const int64_t last = first + kBiasRows < end ? first + kBiasRows : end;
     const int col = blockIdx.y * 256 + lane * 8;
     float acc[8] = {};
@@ -639,12 +739,11 @@ __global__ void __launch_bounds__(256) ragged_bias_part_kernel(const T* __restri
 }
 
 __global__ void __launch_bounds__(256) ragged_bias_sum_kernel(const RaggedArgs g, const float* __restrict__ part, float* __restrict__ db, int max_pieces) {
-    extern __shared__ int32_t plan_s[];
-    const Plan plan = plan_at(plan_s, g.experts);
-    const int32_t* pre = plan.pre;
+    extern __shared__ int32_t begin[];
+    int32_t* pre = begin + g.experts + 1;
     chain_release();
     chain_wait();
-    if (threadIdx.x < 32) make_plan<kBiasPieces>(g, plan, threadIdx.x);
+    if (threadIdx.x < 32) bias_pieces(g, begin, pre, threadIdx.x);
     __syncthreads();
     const int e = blockIdx.x;
     const int c = blockIdx.y * 256 + threadIdx.x;
@@ -672,7 +771,7 @@ bool make_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, 
 int pairs_here() { return device_info().sm_count / 2; }
 
 size_t smem_of(int stages, int experts) {
-    return 1024 + static_cast<size_t>(stages) * kStageBytes + kEpiWarps * kBoxBytes + (static_cast<size_t>(experts) + 1) * 8;
+    return 1024 + static_cast<size_t>(stages) * kStageBytes + kEpiWarps * kBoxBytes + line_bytes(experts);
 }
 
 template <typename T, int MODE, bool RES>
@@ -727,10 +826,13 @@ int weights_of(const void* x, const void* dy, RaggedArgs g, cudaStream_t st) {
     const int pairs = pairs_here();
     const int code = launch_pairs<T, kWeights, false>(ta, tb, to, g, pairs, st);
     if (code != TB200_OK || g.partial == nullptr) return code;
-    launch_chained(ragged_join_kernel<T>, dim3(pairs - 1, kTile / 32), 256, (g.experts + 1) * 8, st, g, pairs);
+    launch_chained(ragged_join_kernel<T>, dim3(pairs, kTile / 32), 256, 0, st, g, pairs);
     count_launch();
     return launch_status();
 }
+
+// floats of the workspace for shared tiles: their descriptions and the partial tiles
+int64_t share_floats(int64_t T) { return T >= kShareRows ? static_cast<int64_t>(pairs_here()) * (8 + 2 * kPartFloats) : 0; }
 
 int64_t bias_most_pieces(int64_t T, int32_t experts) { return T / kBiasRows + (experts < T ? experts : T); }
 
@@ -787,8 +889,7 @@ extern "C" int tb200_ragged_gemm_dgrad(const void* dy, const void* w, const int3
 extern "C" int64_t tb200_ragged_wgrad_workspace_bytes(int32_t experts, int64_t T, int32_t N, int32_t K) {
     using namespace tb200;
     if (checked(experts, T, N, K, TB200_BF16) != TB200_OK || experts == 0) return 0;
-    const int64_t parts = T >= kShareRows ? static_cast<int64_t>(pairs_here()) * 2 * kPartFloats : 0;
-    return 4 * (parts + bias_most_pieces(T, experts) * N);
+    return 4 * (share_floats(T) + bias_most_pieces(T, experts) * N);
 }
 
 extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int32_t* offsets, void* dw, float* db, float* workspace, int32_t experts,
@@ -816,10 +917,13 @@ extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int3
     g.T = T;
     g.cols = K;
     g.n = N;
-    g.partial = T >= kShareRows ? workspace : nullptr;
+    if (T >= kShareRows) {
+        g.pieces = reinterpret_cast<int4*>(workspace);
+        g.partial = workspace + pairs_here() * 8;
+    }
     if (dw != nullptr) code = dtype == TB200_BF16 ? weights_of<__nv_bfloat16>(x, dy, g, st) : weights_of<__half>(x, dy, g, st);
     if (code != TB200_OK || db == nullptr) return code;
-    float* part = workspace + (T >= kShareRows ? static_cast<int64_t>(pairs_here()) * 2 * kPartFloats : 0);
+    float* part = workspace + share_floats(T);
     const int pieces = static_cast<int>(bias_most_pieces(T, experts));
     const dim3 grid(pieces, (N + 255) / 256);
     const size_t smem = (static_cast<size_t>(experts) + 1) * 8;
