@@ -113,29 +113,34 @@ __device__ __forceinline__ int expert_of(const int32_t* pre, int experts, int64_
     return lo;
 }
 __device__ __forceinline__ int row_tiles(const int32_t* begin, int e) { return (begin[e + 1] - begin[e] + kTile - 1) / kTile; }
-// 64-row blocks of an expert's weight gradient; one without rows has one: its zeros are written
+// 64-row blocks of an expert's weight gradient, as its tiles' length in the line: at least what writing a tile costs (an expert without
+// rows has its zeros written), which is below 2 kSnap, so that such tiles are not shared
+constexpr int kLeast = 6;
 __device__ __forceinline__ int row_blocks(const int32_t* begin, int e) {
-    const int rows = begin[e + 1] - begin[e];
-    return rows == 0 ? 1 : (rows + kBlock - 1) / kBlock;
+    const int n = (begin[e + 1] - begin[e] + kBlock - 1) / kBlock;
+    return n < kLeast ? kLeast : n;
 }
 
 // How the tiles of the weight gradients are shared out.  All experts have `tiles` tiles, each as long as its expert has blocks.  The
-// experts stand in a line, those whose tiles are no longer than a pair's equal share in front, and their tiles one after
-// the other.  The first `wave_tiles` of the line go round robin, so that the pairs are on the same few experts at a time and read the
-// same rows while these are in the L2; every pair stays within its equal share there.  What lies behind is cut so that
-// all pairs end up with equal shares.
+// experts stand in a line, the long ones in front (but those whose tiles are longer than a pair's equal share at the end), and
+// their tiles one after the other.  The first `wave_tiles` of the line go round robin, so that the pairs are on the same few
+// experts at a time and read the same rows while these are in the L2; every pair stays within its equal share there.
+// What lies behind is cut so that all pairs end up with equal shares.  Measured at 16 experts of 2048 rows, 2048 x 2048: 359 us
+// with one contiguous share for every pair (rows of all experts are in use all the time), 238 so.
 struct Line {
     int32_t* begin;       // [experts + 1] first rows
     int32_t* pre;         // [experts + 1] blocks of one column of tiles before the i-th expert of the line
     int32_t* order;       // [experts] expert numbers in the order of the line
     int64_t* wave_tiles;  // [1]
     int64_t* cut;         // [2] begin and end of this pair's share of the rest
+    int32_t* place;       // [kClasses + 1] while the line is made
 };
-__host__ __device__ __forceinline__ size_t line_bytes(int experts) { return 24 + 4 * (3 * static_cast<size_t>(experts) + 2); }
+constexpr int kClasses = 32;
+__host__ __device__ __forceinline__ size_t line_bytes(int experts) { return 24 + 4 * (3 * static_cast<size_t>(experts) + 2 + kClasses + 1); }
 __device__ __forceinline__ Line line_at(void* smem, int experts) {
     int64_t* w = static_cast<int64_t*>(smem);
     int32_t* p = reinterpret_cast<int32_t*>(w + 3);
-    return Line{p, p + experts + 1, p + 2 * (experts + 1), w, w + 1};
+    return Line{p, p + experts + 1, p + 2 * (experts + 1), w, w + 1, p + 3 * experts + 2};
 }
 // `p` moved to an edge of its tile where it lies near one: a partial tile costs about as much as kSnap blocks
 __device__ __forceinline__ int64_t snapped(const Line& line, int experts, int tiles, int64_t p) {
@@ -162,25 +167,59 @@ __device__ void make_line(const RaggedArgs& g, const Line& line, int tiles, int 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const int64_t total = static_cast<int64_t>(sum) * tiles, share = total / pairs;
-    int placed = 0, shorter = 0, longest = 1;
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int base = 0; base < g.experts; base += 32) {
-            const int e = base + lane;
-            const int nb = e < g.experts ? row_blocks(line.begin, e) : 0;
-            const bool mine = e < g.experts && (nb <= share) == (pass == 0);
-            const uint32_t mask = __ballot_sync(0xffffffffu, mine);
-            if (mine) line.order[placed + __popc(mask & ((1u << lane) - 1))] = e;
-            if (mine && pass == 0) longest = max(longest, nb);
-            placed += __popc(mask);
-        }
-        if (pass == 0) shorter = placed;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+    // the line: a counting sort by length, kClasses steps up to a pair's share, the longest first and those beyond it last
+    const int64_t width = share / kClasses + 1;
+    auto class_of = [&](int e) {
+        const int nb = row_blocks(line.begin, e);
+        return nb > share ? kClasses : kClasses - 1 - static_cast<int>((nb - 1) / width);
+    };
+    for (int c = lane; c <= kClasses; c += 32) line.place[c] = 0;
     __syncwarp();
+    for (int e = lane; e < g.experts; e += 32) atomicAdd(&line.place[class_of(e)], 1);
+    __syncwarp();
+    if (lane == 0) {
+        int at = 0;
+        for (int c = 0; c <= kClasses; ++c) {
+            const int n = line.place[c];
+            line.place[c] = at;
+            at += n;
+        }
+    }
+    __syncwarp();
+    const int shorter = line.place[kClasses];
+    for (int base = 0; base < g.experts; base += 32) {
+        const int e = base + lane;
+        const int c = e < g.experts ? class_of(e) : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, c);
+        const int before = __popc(same & ((1u << lane) - 1));
+        const int at = c < 0 ? 0 : line.place[c];
+        __syncwarp();
+        if (c >= 0) {
+            line.order[at + before] = e;
+            if (before == 0) line.place[c] = at + __popc(same);
+        }
+        __syncwarp();
+    }
     prefix(line.pre, g.experts, lane, [&](int i) { return row_blocks(line.begin, line.order[i]); });
+    // as many rounds as leave every pair within its share: none of a round's tiles is longer than its first one and a class
     const int64_t fit = static_cast<int64_t>(shorter) * tiles / pairs;
-    const int64_t waves = fit < share / longest ? fit : share / longest;
+    int64_t waves = 0, reached = 0;
+    for (bool more = fit > 0; more;) {
+        int64_t length = INT32_MAX;
+        if (waves + lane < fit) {
+            const int i = static_cast<int>((waves + lane) * pairs / tiles);
+            length = line.pre[i + 1] - line.pre[i] + width;
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, length, o);
+            if (lane >= o) length += u;
+        }
+        const int n = __popc(__ballot_sync(0xffffffffu, reached + length <= share));      // lengths are positive: the first n lanes
+        if (n > 0) reached += __shfl_sync(0xffffffffu, length, n - 1);
+        waves += n;
+        more = n == 32;
+    }
     if (lane == 0) *line.wave_tiles = waves * pairs;
     int64_t before = 0;      // blocks of the waves that go to the pairs in front
     const int64_t rest = waves * pairs / tiles;      // the expert that the line's rest begins in
@@ -273,7 +312,8 @@ struct Walk {
             j.a0 = tile / b_tiles * kTile;
             j.b0 = tile % b_tiles * kTile;
             j.m0 = j.begin + static_cast<int64_t>(first) * kBlock;
-            j.blocks = j.end > j.begin ? take : 0;
+            const int blocks = static_cast<int>((j.end - j.begin + kBlock - 1) / kBlock);
+            j.blocks = blocks < take ? blocks : take;
             j.slot = take == nb ? -1 : (first > 0 ? 0 : 1);
             j.last = first + take == nb;
         } else {
@@ -298,12 +338,14 @@ struct Walk {
 // silu(x) = x / (1 + exp(-x))
 __device__ __forceinline__ float silu(float x) { return x * __fdividef(1.0f, 1.0f + __expf(-x)); }
 
-// Sets the contraction rows [valid, 64) of a stage's four chunks to zero, by one warp
+// Contraction rows that an expert's last block is taken for: whole steps of 16, the depth of one MMA
+__device__ __forceinline__ int tail_depth(int valid) { return (valid + 15) & ~15; }
+// Sets the rows [valid, tail_depth(valid)) of a stage's four chunks to zero, by one warp: eight lanes a row
 __device__ __forceinline__ void clear_tail(uint8_t* stage, int valid, int lane) {
-    const int pieces = (kBlock - valid) * 8;
-    for (int i = lane; i < 4 * pieces; i += 32) {
-        const int chunk = i / pieces, r = i - chunk * pieces;
-        *reinterpret_cast<uint4*>(stage + chunk * kChunkBytes + valid * 128 + r * 16) = make_uint4(0u, 0u, 0u, 0u);
+    const int end = tail_depth(valid);
+    for (int r = valid + (lane >> 3); r < end; r += 4) {
+#pragma unroll
+        for (int chunk = 0; chunk < 4; ++chunk) *reinterpret_cast<uint4*>(stage + chunk * kChunkBytes + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -443,9 +485,11 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                 const uint32_t d_tmem = tmem + buf * kTile;
                 for (int b = 0; b < j.blocks; ++b) {
                     if (!mbar_wait_warp(&full_bar[s], ph)) { ok = false; break; }
+                    int depth = kBlock;
                     if (MODE == kWeights) {
                         const int64_t valid = j.end - (j.m0 + static_cast<int64_t>(b) * kBlock);
                         if (valid < kBlock) {
+                            depth = tail_depth(static_cast<int>(valid));
                             asm volatile("fence.acq_rel.cluster;" ::: "memory");      // the other CTA has cleared its half
                             clear_tail(ring + static_cast<size_t>(s) * kStageBytes, static_cast<int>(valid), lane);
                         }
@@ -456,7 +500,7 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                     if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < kBlock / 16; ++k)
-                            mma_f16_ss_pair(d_tmem, da + step_a * k, db + step_b * k, idesc, (b | k) != 0 ? 1u : 0u);
+                            if (MODE != kWeights || k * 16 < depth) mma_f16_ss_pair(d_tmem, da + step_a * k, db + step_b * k, idesc, (b | k) != 0 ? 1u : 0u);
                         tc_commit_pair(&empty_bar[s]);
                     }
                     __syncwarp();
@@ -693,65 +737,88 @@ __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, in
     }
 }
 
-// db[e] = sum of the expert's rows of dy, in two steps of fixed order.  Step one: CTA (x, y) adds up to kBiasRows rows (a piece of
-// one expert) for 256 columns; its eight warps take every eighth row, eight columns a lane.
-constexpr int kBiasRows = 256;
+// db[e] = sum of the expert's rows of dy, in two steps of fixed order.  Step one: CTA (x, y) adds up to kBiasRows rows (a piece of one
+// expert) for blockDim.x * 8 columns; thread (tx, ty) takes eight columns of every blockDim.y-th row, eight loads in flight.
+// Step two adds an expert's pieces, eight threads a column.
+constexpr int kBiasRows = 32;
 __device__ void bias_pieces(const RaggedArgs& g, int32_t* begin, int32_t* pre, int lane) {
     first_rows(g, begin, lane);
     prefix(pre, g.experts, lane, [&](int e) { return (begin[e + 1] - begin[e] + kBiasRows - 1) / kBiasRows; });
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) ragged_bias_part_kernel(const T* __restrict__ dy, const RaggedArgs g, float* __restrict__ part, int max_pieces) {
-    extern __shared__ int32_t begin[];
-    __shared__ float sums[8][256];
+__global__ void __launch_bounds__(256) ragged_bias_part_kernel(const T* __restrict__ dy, const RaggedArgs g, float* __restrict__ part) {
+    extern __shared__ float sums[];                              // [blockDim.y - 1][blockDim.x * 8], then the plan
+    const int width = blockDim.x * 8;
+    int32_t* begin = reinterpret_cast<int32_t*>(sums + (blockDim.y - 1) * width);
     int32_t* pre = begin + g.experts + 1;
     chain_release();
     chain_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) bias_pieces(g, begin, pre, lane);
+    const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+    if (tid < 32) bias_pieces(g, begin, pre, tid);
     __syncthreads();
     const int piece = blockIdx.x;
-    if (piece >= pre[g.experts] || piece >= max_pieces) return;
+    if (piece >= pre[g.experts]) return;
     const int e = expert_of(pre, g.experts, piece);
     const int64_t first = begin[e] + static_cast<int64_t>(piece - pre[e]) * kBiasRows, end = begin[e + 1];
     const int64_t last = first + kBiasRows < end ? first + kBiasRows : end;
-    const int col = blockIdx.y * 256 + lane * 8;
+    const int col = blockIdx.y * width + threadIdx.x * 8;
     float acc[8] = {};
     if (col < g.n) {
-#pragma unroll 4
-        for (int64_t r = first + warp; r < last; r += 8) {
-            float v[8];
-            Vec16<T>::unpack(__ldg(reinterpret_cast<const uint4*>(dy + r * g.n + col)), v);
+        const uint4* at = reinterpret_cast<const uint4*>(dy + (first + threadIdx.y) * g.n + col);
+        const int64_t step = static_cast<int64_t>(blockDim.y) * g.n / 8;
+        for (int64_t r = first + threadIdx.y; r < last; r += 8 * blockDim.y, at += 8 * step) {
+            uint4 raw[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += v[i];
+            for (int u = 0; u < 8; ++u) raw[u] = r + u * static_cast<int>(blockDim.y) < last ? __ldg(at + u * step) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                float v[8];
+                Vec16<T>::unpack(raw[u], v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] += v[i];
+            }
         }
     }
+    if (blockDim.y > 1) {
+        if (threadIdx.y > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sums[warp][lane * 8 + i] = acc[i];
-    __syncthreads();
-    const int c = blockIdx.y * 256 + threadIdx.x;
-    if (c >= g.n) return;
-    float s = 0.f;
+            for (int i = 0; i < 8; ++i) sums[(threadIdx.y - 1) * width + i * blockDim.x + threadIdx.x] = acc[i];
+        }
+        __syncthreads();
+        if (threadIdx.y > 0) return;
+        for (int k = 1; k < static_cast<int>(blockDim.y); ++k) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += sums[k][threadIdx.x];
-    part[static_cast<int64_t>(piece) * g.n + c] = s;
+            for (int i = 0; i < 8; ++i) acc[i] += sums[(k - 1) * width + i * blockDim.x + threadIdx.x];
+        }
+    }
+    if (col >= g.n) return;
+    float4* out = reinterpret_cast<float4*>(part + static_cast<int64_t>(piece) * g.n + col);
+    out[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    out[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
 }
 
-__global__ void __launch_bounds__(256) ragged_bias_sum_kernel(const RaggedArgs g, const float* __restrict__ part, float* __restrict__ db, int max_pieces) {
+__global__ void __launch_bounds__(256) ragged_bias_sum_kernel(const RaggedArgs g, const float* __restrict__ part, float* __restrict__ db) {
     extern __shared__ int32_t begin[];
+    __shared__ float sums[7][32];
     int32_t* pre = begin + g.experts + 1;
     chain_release();
     chain_wait();
-    if (threadIdx.x < 32) bias_pieces(g, begin, pre, threadIdx.x);
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    if (ty == 0) bias_pieces(g, begin, pre, tx);
     __syncthreads();
     const int e = blockIdx.x;
-    const int c = blockIdx.y * 256 + threadIdx.x;
-    if (c >= g.n) return;
+    const int c = blockIdx.y * 32 + tx;
     float s = 0.f;
-    const int last = min(pre[e + 1], max_pieces);
+    if (c < g.n) {
 #pragma unroll 4
-    for (int p = pre[e]; p < last; ++p) s += part[static_cast<int64_t>(p) * g.n + c];
+        for (int p = pre[e] + ty; p < pre[e + 1]; p += 8) s += part[static_cast<int64_t>(p) * g.n + c];
+    }
+    if (ty > 0) sums[ty - 1][tx] = s;
+    __syncthreads();
+    if (ty > 0 || c >= g.n) return;
+#pragma unroll
+    for (int k = 0; k < 7; ++k) s += sums[k][tx];
     db[static_cast<int64_t>(e) * g.n + c] = s;
 }
 
@@ -814,7 +881,7 @@ int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bo
     return launch_pairs<T, kRows, false>(ta, tb, to, g, pairs, st);
 }
 
-// rows from which on a tile can be shared by pairs: below, no expert has 2 kSnap blocks
+// rows from which on a tile can be shared by pairs: with fewer, no expert has 2 kSnap blocks
 constexpr int64_t kShareRows = 2 * kSnap * kBlock;
 
 template <typename T>
@@ -924,14 +991,16 @@ extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int3
     if (dw != nullptr) code = dtype == TB200_BF16 ? weights_of<__nv_bfloat16>(x, dy, g, st) : weights_of<__half>(x, dy, g, st);
     if (code != TB200_OK || db == nullptr) return code;
     float* part = workspace + share_floats(T);
-    const int pieces = static_cast<int>(bias_most_pieces(T, experts));
-    const dim3 grid(pieces, (N + 255) / 256);
-    const size_t smem = (static_cast<size_t>(experts) + 1) * 8;
+    // as many threads along the columns as there are octets (a whole number of warps, at most the CTA), the others along the rows
+    int tx = 32;
+    while (tx < 256 && tx * 8 < N) tx *= 2;
+    const dim3 grid(static_cast<unsigned>(bias_most_pieces(T, experts)), (N + tx * 8 - 1) / (tx * 8)), block(tx, 256 / tx);
+    const size_t plan = (static_cast<size_t>(experts) + 1) * 8, smem = static_cast<size_t>(256 / tx - 1) * tx * 8 * 4 + plan;
     if (dtype == TB200_BF16)
-        launch_chained(ragged_bias_part_kernel<__nv_bfloat16>, grid, 256, smem, st, static_cast<const __nv_bfloat16*>(dy), g, part, pieces);
+        launch_chained(ragged_bias_part_kernel<__nv_bfloat16>, grid, block, smem, st, static_cast<const __nv_bfloat16*>(dy), g, part);
     else
-        launch_chained(ragged_bias_part_kernel<__half>, grid, 256, smem, st, static_cast<const __half*>(dy), g, part, pieces);
-    launch_chained(ragged_bias_sum_kernel, dim3(experts, (N + 255) / 256), 256, smem, st, g, part, db, pieces);
+        launch_chained(ragged_bias_part_kernel<__half>, grid, block, smem, st, static_cast<const __half*>(dy), g, part);
+    launch_chained(ragged_bias_sum_kernel, dim3(experts, (N + 31) / 32), 256, plan, st, g, part, db);
     count_launch();
     count_launch();
     return launch_status();
