@@ -737,82 +737,81 @@ __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, in
     }
 }
 
-// db[e] = sum of the expert's rows of dy, in two steps of fixed order.  Step one: CTA (x, y) adds up to kBiasRows rows (a piece of one
-// expert) for blockDim.x * 8 columns; thread (tx, ty) takes eight columns of every blockDim.y-th row, eight loads in flight.
-// Step two adds an expert's pieces, eight threads a column.
-constexpr int kBiasRows = 32;
-__device__ void bias_pieces(const RaggedArgs& g, int32_t* begin, int32_t* pre, int lane) {
-    first_rows(g, begin, lane);
-    prefix(pre, g.experts, lane, [&](int e) { return (begin[e + 1] - begin[e] + kBiasRows - 1) / kBiasRows; });
-}
-
+// db[e] = sum of the expert's rows of dy, in two steps of fixed order.  Step one: CTA (x, y) adds the rows of chunk x, `chunk` rows
+// of the matrix, for blockDim.x * 8 columns, and leaves a partial sum for every expert that has rows among them; that of
+// expert e stands in row x + e of the table, which no other pair of chunk and expert has, for both grow along the matrix.
+// Thread (tx, ty) takes eight columns of every blockDim.y-th row, eight loads in flight.  As many chunks as CTAs fit the chip:
+// pieces of 32 rows of one expert, a CTA each, took 42 us instead of 24 for 32768 x 2048, start-up and waves of CTAs.
+// Step two adds an expert's partial sums, eight threads a column.
 template <typename T>
-__global__ void __launch_bounds__(256) ragged_bias_part_kernel(const T* __restrict__ dy, const RaggedArgs g, float* __restrict__ part) {
-    extern __shared__ float sums[];                              // [blockDim.y - 1][blockDim.x * 8], then the plan
+__global__ void __launch_bounds__(256) ragged_bias_part_kernel(const T* __restrict__ dy, const RaggedArgs g, float* __restrict__ part, int64_t chunk) {
+    extern __shared__ float sums[];                              // [blockDim.y - 1][blockDim.x * 8], then the first rows
     const int width = blockDim.x * 8;
     int32_t* begin = reinterpret_cast<int32_t*>(sums + (blockDim.y - 1) * width);
-    int32_t* pre = begin + g.experts + 1;
     chain_release();
     chain_wait();
     const int tid = threadIdx.y * blockDim.x + threadIdx.x;
-    if (tid < 32) bias_pieces(g, begin, pre, tid);
+    if (tid < 32) first_rows(g, begin, tid);
     __syncthreads();
-    const int piece = blockIdx.x;
-    if (piece >= pre[g.experts]) return;
-    const int e = expert_of(pre, g.experts, piece);
-    const int64_t first = begin[e] + static_cast<int64_t>(piece - pre[e]) * kBiasRows, end = begin[e + 1];
-    const int64_t last = first + kBiasRows < end ? first + kBiasRows : end;
+    const int64_t from = max(blockIdx.x * chunk, static_cast<int64_t>(begin[0]));
+    const int64_t to = min((blockIdx.x + 1) * chunk, static_cast<int64_t>(begin[g.experts]));
     const int col = blockIdx.y * width + threadIdx.x * 8;
-    float acc[8] = {};
-    if (col < g.n) {
-        const uint4* at = reinterpret_cast<const uint4*>(dy + (first + threadIdx.y) * g.n + col);
-        const int64_t step = static_cast<int64_t>(blockDim.y) * g.n / 8;
-        for (int64_t r = first + threadIdx.y; r < last; r += 8 * blockDim.y, at += 8 * step) {
-            uint4 raw[8];
+    const int by = blockDim.y;
+    if (from >= to) return;
+    for (int e = expert_of(begin, g.experts, from); e < g.experts && begin[e] < to; ++e) {
+        const int64_t first = max(from, static_cast<int64_t>(begin[e])), last = min(to, static_cast<int64_t>(begin[e + 1]));
+        if (first >= last) continue;
+        float acc[8] = {};
+        if (col < g.n) {
+            for (int64_t r = first + threadIdx.y; r < last; r += 8 * by) {
+                uint4 raw[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) raw[u] = r + u * static_cast<int>(blockDim.y) < last ? __ldg(at + u * step) : make_uint4(0u, 0u, 0u, 0u);
+                for (int u = 0; u < 8; ++u)
+                    raw[u] = r + u * by < last ? __ldg(reinterpret_cast<const uint4*>(dy + (r + u * by) * g.n + col)) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                float v[8];
-                Vec16<T>::unpack(raw[u], v);
+                for (int u = 0; u < 8; ++u) {
+                    float v[8];
+                    Vec16<T>::unpack(raw[u], v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] += v[i];
+                    for (int i = 0; i < 8; ++i) acc[i] += v[i];
+                }
             }
         }
-    }
-    if (blockDim.y > 1) {
-        if (threadIdx.y > 0) {
+        if (by > 1) {
+            if (threadIdx.y > 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sums[(threadIdx.y - 1) * width + i * blockDim.x + threadIdx.x] = acc[i];
-        }
-        __syncthreads();
-        if (threadIdx.y > 0) return;
-        for (int k = 1; k < static_cast<int>(blockDim.y); ++k) {
+                for (int i = 0; i < 8; ++i) sums[(threadIdx.y - 1) * width + i * blockDim.x + threadIdx.x] = acc[i];
+            }
+            __syncthreads();
+            for (int k = 1; k < by && threadIdx.y == 0; ++k) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += sums[(k - 1) * width + i * blockDim.x + threadIdx.x];
+                for (int i = 0; i < 8; ++i) acc[i] += sums[(k - 1) * width + i * blockDim.x + threadIdx.x];
+            }
+            __syncthreads();
+        }
+        if (threadIdx.y == 0 && col < g.n) {
+            float4* out = reinterpret_cast<float4*>(part + (static_cast<int64_t>(blockIdx.x) + e) * g.n + col);
+            out[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            out[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
         }
     }
-    if (col >= g.n) return;
-    float4* out = reinterpret_cast<float4*>(part + static_cast<int64_t>(piece) * g.n + col);
-    out[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    out[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
 }
 
-__global__ void __launch_bounds__(256) ragged_bias_sum_kernel(const RaggedArgs g, const float* __restrict__ part, float* __restrict__ db) {
+__global__ void __launch_bounds__(256) ragged_bias_sum_kernel(const RaggedArgs g, const float* __restrict__ part, float* __restrict__ db, int64_t chunk) {
     extern __shared__ int32_t begin[];
     __shared__ float sums[7][32];
-    int32_t* pre = begin + g.experts + 1;
     chain_release();
     chain_wait();
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    if (ty == 0) bias_pieces(g, begin, pre, tx);
+    if (ty == 0) first_rows(g, begin, tx);
     __syncthreads();
     const int e = blockIdx.x;
     const int c = blockIdx.y * 32 + tx;
     float s = 0.f;
-    if (c < g.n) {
+    if (c < g.n && begin[e + 1] > begin[e]) {
+        const int last = static_cast<int>((begin[e + 1] - 1) / chunk);
 #pragma unroll 4
-        for (int p = pre[e] + ty; p < pre[e + 1]; p += 8) s += part[static_cast<int64_t>(p) * g.n + c];
+        for (int x = static_cast<int>(begin[e] / chunk) + ty; x <= last; x += 8) s += part[(static_cast<int64_t>(x) + e) * g.n + c];
     }
     if (ty > 0) sums[ty - 1][tx] = s;
     __syncthreads();
@@ -901,7 +900,22 @@ int weights_of(const void* x, const void* dy, RaggedArgs g, cudaStream_t st) {
 // floats of the workspace for shared tiles: their descriptions and the partial tiles
 int64_t share_floats(int64_t T) { return T >= kShareRows ? static_cast<int64_t>(pairs_here()) * (8 + 2 * kPartFloats) : 0; }
 
-int64_t bias_most_pieces(int64_t T, int32_t experts) { return T / kBiasRows + (experts < T ? experts : T); }
+// How the sum of the bias gradient's rows is laid over the chip: as many threads along the columns as there are octets (whole warps, at
+// most the CTA), the others along the rows; four CTAs an SM, at least 16 rows each
+struct BiasShape {
+    int tx, columns;      // threads along the columns, CTAs along them
+    int64_t chunk, chunks;
+};
+BiasShape bias_shape(int64_t T, int32_t N) {
+    BiasShape b{32, 0, 16, 0};
+    while (b.tx < 256 && b.tx * 8 < N) b.tx *= 2;
+    b.columns = (N + b.tx * 8 - 1) / (b.tx * 8);
+    const int64_t ctas = static_cast<int64_t>(device_info().sm_count) * 4 / b.columns;
+    const int64_t rows = ctas < 1 ? T : (T + ctas - 1) / ctas;
+    if (rows > b.chunk) b.chunk = rows;
+    b.chunks = (T + b.chunk - 1) / b.chunk;
+    return b;
+}
 
 }  // namespace
 }  // namespace tb200
@@ -956,7 +970,7 @@ extern "C" int tb200_ragged_gemm_dgrad(const void* dy, const void* w, const int3
 extern "C" int64_t tb200_ragged_wgrad_workspace_bytes(int32_t experts, int64_t T, int32_t N, int32_t K) {
     using namespace tb200;
     if (checked(experts, T, N, K, TB200_BF16) != TB200_OK || experts == 0) return 0;
-    return 4 * (share_floats(T) + bias_most_pieces(T, experts) * N);
+    return 4 * (share_floats(T) + (bias_shape(T, N).chunks + experts) * N);
 }
 
 extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int32_t* offsets, void* dw, float* db, float* workspace, int32_t experts,
@@ -991,16 +1005,14 @@ extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int3
     if (dw != nullptr) code = dtype == TB200_BF16 ? weights_of<__nv_bfloat16>(x, dy, g, st) : weights_of<__half>(x, dy, g, st);
     if (code != TB200_OK || db == nullptr) return code;
     float* part = workspace + share_floats(T);
-    // as many threads along the columns as there are octets (a whole number of warps, at most the CTA), the others along the rows
-    int tx = 32;
-    while (tx < 256 && tx * 8 < N) tx *= 2;
-    const dim3 grid(static_cast<unsigned>(bias_most_pieces(T, experts)), (N + tx * 8 - 1) / (tx * 8)), block(tx, 256 / tx);
-    const size_t plan = (static_cast<size_t>(experts) + 1) * 8, smem = static_cast<size_t>(256 / tx - 1) * tx * 8 * 4 + plan;
+    const BiasShape b = bias_shape(T, N);
+    const dim3 grid(static_cast<unsigned>(b.chunks), b.columns), block(b.tx, 256 / b.tx);
+    const size_t rows = (static_cast<size_t>(experts) + 1) * 4, smem = static_cast<size_t>(256 / b.tx - 1) * b.tx * 8 * 4 + rows;
     if (dtype == TB200_BF16)
-        launch_chained(ragged_bias_part_kernel<__nv_bfloat16>, grid, block, smem, st, static_cast<const __nv_bfloat16*>(dy), g, part);
+        launch_chained(ragged_bias_part_kernel<__nv_bfloat16>, grid, block, smem, st, static_cast<const __nv_bfloat16*>(dy), g, part, b.chunk);
     else
-        launch_chained(ragged_bias_part_kernel<__half>, grid, block, smem, st, static_cast<const __half*>(dy), g, part);
-    launch_chained(ragged_bias_sum_kernel, dim3(experts, (N + 31) / 32), 256, plan, st, g, part, db);
+        launch_chained(ragged_bias_part_kernel<__half>, grid, block, smem, st, static_cast<const __half*>(dy), g, part, b.chunk);
+    launch_chained(ragged_bias_sum_kernel, dim3(experts, (N + 31) / 32), 256, rows, st, g, part, db, b.chunk);
     count_launch();
     count_launch();
     return launch_status();
