@@ -39,14 +39,6 @@ struct NarrowArgs {
     uint32_t tmem_cols;
 };
 
-__device__ __forceinline__ float ld_peer(uint32_t smem_addr, uint32_t rank) {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
-    return v;
-}
-
 // Sixteen outputs of one column, rows `step` apart: all residual loads before the first store (`out` may be the residual)
 __device__ __forceinline__ void load_residual(const NarrowArgs& g, int64_t at, int rows, int step, float (&res)[16]) {
 #pragma unroll

@@ -23,12 +23,12 @@
 // more pairs share leaves fp32 partial tiles in a workspace, which `ragged_join_kernel` adds in the order of the pairs.
 //
 // Every wait on an mbarrier is bounded; a wait that gives up raises the status word and all roles drain through the final barrier.
-#include "tb200_common.cuh"
-#include "tb200_tmap.cuh"
+#include "ragged.cuh"
 #include "tc_pair.cuh"
 
 namespace tb200 {
 void count_launch();
+int ragged_few(const void* rows, const void* w, const RaggedArgs& g, int32_t N, int32_t K, bool grads, bool bf16, cudaStream_t st);
 
 namespace {
 
@@ -44,74 +44,10 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + kEpiWarps * 32;
 constexpr uint32_t kBoxBytes = 32 * 128;                  // an epilogue warp's staging box: 32 rows x 64 columns
 constexpr uint32_t kTmemCols = 512;
-constexpr int kMaxExperts = 2048;
 constexpr int kSnap = 4;
 constexpr int64_t kPartFloats = int64_t(kTile) * kTile;   // of a partial tile
 constexpr size_t kSmemLimit = 227 * 1024 - 512;           // less the static part
 
-struct RaggedArgs {
-    const int32_t* offsets;     // [experts + 1]
-    const float* bias;          // [experts, cols] or NULL (rows)
-    const void* residual;       // [T, cols] or NULL (rows)
-    void* out;                  // [T, cols], or [experts, n, k] (weights)
-    float* partial;             // [pairs][2] partial tiles, NULL: tiles are never shared (weights)
-    int4* pieces;               // [pairs][2] what they are part of: expert (-1: nothing), first row and column of the tile, last piece?
-    int32_t* status;
-    int32_t experts, stages;
-    int64_t T;
-    int32_t cols;               // of a result row
-    int32_t depth;              // contracted length (rows, row grads)
-    int32_t n;                  // rows of a weight gradient
-    int32_t silu;
-    int32_t clear;              // rows of no expert are set to zero
-};
-
-// Where every expert's rows begin, by one warp; the offsets come from the kernel in front.  An offset outside [0, T] is moved to
-// the nearer end and one that lies before an earlier one counts as that one, so that no two experts share a row.
-__device__ void first_rows(const RaggedArgs& g, int32_t* begin, int lane) {
-    int32_t top = 0;
-    for (int base = 0; base <= g.experts; base += 32) {
-        int32_t v = 0;
-        if (base + lane <= g.experts) v = __ldcg(g.offsets + base + lane);
-        v = v < 0 ? 0 : (v > g.T ? static_cast<int32_t>(g.T) : v);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v = max(v, u);
-        }
-        v = max(v, top);
-        if (base + lane <= g.experts) begin[base + lane] = v;
-        top = __shfl_sync(0xffffffffu, v, 31);
-    }
-    __syncwarp();
-}
-// pre[i] = sum of units(0 .. i - 1), by one warp
-template <typename F>
-__device__ void prefix(int32_t* pre, int n, int lane, F units) {
-    int32_t sum = 0;
-    for (int base = 0; base < n; base += 32) {
-        int32_t v = base + lane < n ? units(base + lane) : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += u;
-        }
-        if (base + lane < n) pre[base + lane + 1] = sum + v;
-        sum += __shfl_sync(0xffffffffu, v, 31);
-    }
-    if (lane == 0) pre[0] = 0;
-    __syncwarp();
-}
-// the last i with pre[i] <= unit: the expert whose units hold `unit`
-__device__ __forceinline__ int expert_of(const int32_t* pre, int experts, int64_t unit) {
-    int lo = 0, hi = experts;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (pre[mid] <= unit) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
 __device__ __forceinline__ int row_tiles(const int32_t* begin, int e) { return (begin[e + 1] - begin[e] + kTile - 1) / kTile; }
 // 64-row blocks of an expert's weight gradient, as its tiles' length in the line: at least what writing a tile costs (an expert without
 // rows has its zeros written), which is below 2 kSnap, so that such tiles are not shared
@@ -335,8 +271,6 @@ struct Walk {
     }
 };
 
-// silu(x) = x / (1 + exp(-x))
-__device__ __forceinline__ float silu(float x) { return x * __fdividef(1.0f, 1.0f + __expf(-x)); }
 
 // Contraction rows that an expert's last block is taken for: whole steps of 16, the depth of one MMA
 __device__ __forceinline__ int tail_depth(int valid) { return (valid + 15) & ~15; }
@@ -822,18 +756,6 @@ __global__ void __launch_bounds__(256) ragged_bias_sum_kernel(const RaggedArgs g
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// a matrix or a stack of matrices of 16-bit values, boxes of box_rows x 128 bytes
-bool make_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t stack, uint32_t box_rows) {
-    const auto fn = encode_fn();
-    if (fn == nullptr) return false;
-    const cuuint64_t dims[3] = {2 * cols, rows, stack};
-    const cuuint64_t strides[2] = {2 * cols, 2 * cols * rows};
-    const cuuint32_t box[3] = {128, box_rows, 1};
-    const cuuint32_t elem[3] = {1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, stack == 0 ? 2 : 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 int pairs_here() { return device_info().sm_count / 2; }
 
 size_t smem_of(int stages, int experts) {
@@ -864,15 +786,21 @@ int checked(int32_t experts, int64_t T, int32_t N, int32_t K, int dtype) {
 }
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
+// Rows an expert up to which the kernel of few rows is taken.  Measured, few rows / pairs, in us: 16 experts, 512 -> 2048, of 32 rows 9.1 /
+// 13.7, of 64 12.3 / 14.0, of 128 15.2 / 14.3, their row gradients 12.2 / 17.4, 18.1 / 17.6, 24.5 / 18.4; 64 experts of 64 rows 30.8 / 40.5
+// and 35.2 / 35.1, of 192 rows 53 / 49 and 56 / 49.
+constexpr int kFewRows = 64;
+
 template <typename T>
 int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bool grads, cudaStream_t st) {
     CUtensorMap ta, tb, to;
     const uint64_t rows = static_cast<uint64_t>(g.T);
     const int32_t in = grads ? N : K, out = grads ? K : N;
-    if (!make_map(&ta, x, in, rows, 0, 128) || !make_map(&tb, w, K, N, g.experts, grads ? 64 : 128) || !make_map(&to, g.out, out, rows, 0, 32))
-        return TB200_ERR_DRIVER;
     g.cols = out;
     g.depth = in;
+    if (g.T <= kFewRows * static_cast<int64_t>(g.experts)) return ragged_few(x, w, g, N, K, grads, std::is_same<T, __nv_bfloat16>::value, st);
+    if (!make_map(&ta, x, in, rows, 0, 128) || !make_map(&tb, w, K, N, g.experts, grads ? 64 : 128) || !make_map(&to, g.out, out, rows, 0, 32))
+        return TB200_ERR_DRIVER;
     const int64_t most = (g.T / kTile + g.experts) * ((out + kTile - 1) / kTile);
     const int pairs = static_cast<int>(most < pairs_here() ? most : pairs_here());
     if (grads) return launch_pairs<T, kRowGrads, false>(ta, tb, to, g, pairs, st);
