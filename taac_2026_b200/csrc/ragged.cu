@@ -788,7 +788,8 @@ bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0
 
 // Rows an expert up to which the kernel of few rows is taken.  Measured, few rows / pairs, in us: 16 experts, 512 -> 2048, of 32 rows 9.1 /
 // 13.7, of 64 12.3 / 14.0, of 128 15.2 / 14.3, their row gradients 12.2 / 17.4, 18.1 / 17.6, 24.5 / 18.4; 64 experts of 64 rows 30.8 / 40.5
-// and 35.2 / 35.1, of 192 rows 53 / 49 and 56 / 49.
+// and 35.2 / 35.1, of 192 rows 53 / 49 and 56 / 49.  It is taken as well where its 64-row units are no more than the pairs, which
+// start more slowly: 2 experts of 200 rows, 256 -> 256, 5.2 / 7.6; one of 256 rows, 512 -> 512, 7.2 / 8.8.
 constexpr int kFewRows = 64;
 
 template <typename T>
@@ -798,7 +799,8 @@ int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bo
     const int32_t in = grads ? N : K, out = grads ? K : N;
     g.cols = out;
     g.depth = in;
-    if (g.T <= kFewRows * static_cast<int64_t>(g.experts)) return ragged_few(x, w, g, N, K, grads, std::is_same<T, __nv_bfloat16>::value, st);
+    const int64_t few_units = (g.T / 64 + (g.experts + 1) / 2) * ((out + 127) / 128);
+    if (g.T <= kFewRows * static_cast<int64_t>(g.experts) || few_units <= pairs_here()) return ragged_few(x, w, g, N, K, grads, std::is_same<T, __nv_bfloat16>::value, st);
     if (!make_map(&ta, x, in, rows, 0, 128) || !make_map(&tb, w, K, N, g.experts, grads ? 64 : 128) || !make_map(&to, g.out, out, rows, 0, 32))
         return TB200_ERR_DRIVER;
     const int64_t most = (g.T / kTile + g.experts) * ((out + kTile - 1) / kTile);
