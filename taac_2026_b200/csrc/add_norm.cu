@@ -105,51 +105,56 @@ add_norm_kernel(const FwdArgs<T> a) {
         const int64_t row = base + sub;
         const bool live = row < a.rows;
         if (!AHEAD) fetch(row);
-        float t[OPT][8];
-        float ss = 0.f;
+        float2 t[OPT][4];
+        float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < OPT; ++j) {
-            float r[8];
-            nx[j].unpack(t[j]);
-            nr[j].unpack(r);
+            float2 r[4];
+            nx[j].unpack2(t[j]);
+            nr[j].unpack2(r);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                t[j][e] += r[e];
-                ss = fmaf(t[j][e], t[j][e], ss);
+            for (int e = 0; e < 4; ++e) {
+                t[j][e] = __fadd2_rn(t[j][e], r[e]);
+                ss = __ffma2_rn(t[j][e], t[j][e], ss);
             }
         }
         if (AHEAD) fetch(row + step);
-        const float s = rsqrtf(row_sum<G>(make_float2(ss, 0.f), slots[parity], 0, blockDim.x >> 5).x * inv_cols + a.eps);
+        const float s = rsqrtf(row_sum<G>(make_float2(ss.x + ss.y, 0.f), slots[parity], 0, blockDim.x >> 5).x * inv_cols + a.eps);
+        const float2 s2 = make_float2(s, s);
 #pragma unroll
         for (int j = 0; j < OPT; ++j) {
             const int c = lg + j * lanes;
             const bool in = live && c < octets;
             const int64_t at = row * a.cols + static_cast<int64_t>(c) * 8;
-            if (in && a.total != nullptr) Octet<T>::store(a.total + at, t[j]);
-            float w[8];
-            gm[j].unpack(w);
+            if (in && a.total != nullptr) Octet<T>::store2(a.total + at, t[j]);
+            float2 w[4];
+            gm[j].unpack2(w);
             float amax = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                t[j][e] = t[j][e] * s * w[e];
-                if (SC != kNoQuant) amax = fmaxf(amax, fabsf(t[j][e]));
+            for (int e = 0; e < 4; ++e) {
+                t[j][e] = __fmul2_rn(__fmul2_rn(t[j][e], s2), w[e]);
+                if (SC != kNoQuant) amax = fmaxf(amax, fmaxf(fabsf(t[j][e].x), fabsf(t[j][e].y)));
             }
-            if (in && a.normed != nullptr) Octet<T>::store(a.normed + at, t[j]);
+            if (in && a.normed != nullptr) Octet<T>::store2(a.normed + at, t[j]);
             if (SC != kNoQuant) {                            // columns are whole blocks: 16 neighbouring lanes hold one
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                 float inv, scale = 1.0f;
                 uint32_t byte = 0;
                 if (SC == kAmax) {                           // the rule of tb200_quant_act_1x128, on the unrounded n
-                    scale = amax > 0.f ? amax / 448.0f : 1.0f;
-                    inv = 1.0f / scale;
+                    // the product and the quick quotient are within 2^-22: every lane forms them, a division would cost a quarter
+                    // of the kernel's instructions.  A block of subnormal values keeps a finite factor, for its zeros.
+                    scale = amax > 0.f ? amax * (1.0f / 448.0f) : 1.0f;
+                    inv = amax > 0.f ? fminf(__fdividef(448.0f, amax), 3.0e38f) : 1.0f;
                 } else {
                     byte = pow2_scale(amax, &inv);
                 }
+                const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[j][e] = __fmul2_rn(t[j][e], inv2);
                 if (in) {
                     *reinterpret_cast<uint2*>(a.q + (at >> 2)) =
-                        make_uint2(pack_e4m3x4(t[j][0] * inv, t[j][1] * inv, t[j][2] * inv, t[j][3] * inv),
-                                   pack_e4m3x4(t[j][4] * inv, t[j][5] * inv, t[j][6] * inv, t[j][7] * inv));
+                        make_uint2(pack_e4m3x4(t[j][0].x, t[j][0].y, t[j][1].x, t[j][1].y), pack_e4m3x4(t[j][2].x, t[j][2].y, t[j][3].x, t[j][3].y));
                     if ((c & 15) == 0) {
                         const int blocks = a.cols >> 7, b = c >> 4;
                         if (SC == kAmax) {

@@ -222,6 +222,26 @@ struct Octet {
             for (int e = 0; e < N; ++e) f[i * N + e] = g[e];
         }
     }
+    __device__ void unpack2(float2 (&f)[4]) const {
+        constexpr int N = Vec16<T>::N / 2;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float2 g[N];
+            Vec16<T>::unpack2(v[i], g);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[i * N + e] = g[e];
+        }
+    }
+    static __device__ void store2(T* p, const float2 (&f)[4]) {
+        constexpr int N = Vec16<T>::N / 2;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            float2 g[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) g[e] = f[i * N + e];
+            *(reinterpret_cast<uint4*>(p) + i) = Vec16<T>::pack2(g);
+        }
+    }
     static __device__ void store(T* p, const float (&f)[8]) {
         constexpr int N = Vec16<T>::N;
 #pragma unroll
