@@ -11,8 +11,12 @@
 //
 // Bound by HBM: each value is read and written once.  A lane works on an octet (8 columns), 16 neighbouring lanes hold a
 // block of 128 columns, whose largest value is found by four shuffles; a lane has kUnroll octets of different places in
-// flight.  sig(g) = 1 / (1 + exp(-g)) in fp32 on the special-function unit (exp to 2 ulp of 2^x, a reciprocal): far below the
-// rounding of a 16-bit result; an fp32 result takes expf and a division.
+// flight.  Instructions are what competes with the bytes: maxima of bits, packed arithmetic and places without divisions took the
+// gated forward pass of 32768 x 2048 bf16 (541 MB) from 103 to 93 us; its backward pass (675 MB) takes 105.  sig(g) =
+// 1 / (1 + exp(-g)) in fp32 on the special-function unit (__expf, a reciprocal to 1 ulp): far below the rounding of a 16-bit
+// result; an fp32 result takes expf and a division.
+#include <type_traits>
+
 #include "quant.cuh"
 #include "tb200_common.cuh"
 
@@ -28,28 +32,100 @@ constexpr int kUnroll = 2;
 template <typename T>
 __device__ __forceinline__ float sigmoid(float g) {
     if (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));
-    return __fdividef(1.0f, 1.0f + __expf(-g));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-g)));
+    return r;
 }
 
-// e4m3 values and scale of the 128 columns that this lane's 16 neighbours hold; all 32 lanes call it
-__device__ __forceinline__ uint2 keep(float (&x)[8], float* scale) {
-    float amax = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float m = fabsf(x[e]);
-        const bool finite = m <= 3.402823466e38f;
-        if (!finite) x[e] = __int_as_float(0x7FC00000);
-        amax = fmaxf(amax, finite ? m : 0.f);
+// ---- largest value of a block.  |x| of every type orders as its bits do, infinity and NaN on top, so the maximum is taken of
+// integers: two 16-bit values at a time, and those of the gate's and the value's block in the halves of one word, which one chain
+// of shuffles reduces.
+template <typename T>
+struct Bits {      // 16-bit types: (maximum, 0) as a word
+    static constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+    static __device__ uint32_t max_of(const Octet<T>& o) {
+        const uint4 v = o.v[0];
+        const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+        return max(m & 0xFFFFu, m >> 16);
     }
+    static __device__ float value(uint32_t bits) {
+        const uint16_t b = static_cast<uint16_t>(bits);
+        return to_float<T>(*reinterpret_cast<const T*>(&b));
+    }
+};
+template <>
+struct Bits<float> {
+    static constexpr uint32_t kInf = 0x7F800000u;
+    static __device__ uint32_t max_of(const Octet<float>& o) {
+        uint32_t m = 0;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float2 s = exact_pow2_scale(amax);
-    *scale = s.x;
-    return make_uint2(pack_e4m3x4(x[0] * s.y, x[1] * s.y, x[2] * s.y, x[3] * s.y),
-                      pack_e4m3x4(x[4] * s.y, x[5] * s.y, x[6] * s.y, x[7] * s.y));
+        for (int i = 0; i < 2; ++i)
+            m = max(m, max(max(o.v[i].x & 0x7FFFFFFFu, o.v[i].y & 0x7FFFFFFFu), max(o.v[i].z & 0x7FFFFFFFu, o.v[i].w & 0x7FFFFFFFu)));
+        return m;
+    }
+    static __device__ float value(uint32_t bits) { return __uint_as_float(bits); }
+};
+
+// the blocks' largest bits, of gate and value, among the 16 neighbours; all 32 lanes call it
+template <typename T, bool TWO>
+__device__ __forceinline__ uint2 block_max(const Octet<T>& g, const Octet<T>& v) {
+    uint32_t a = Bits<T>::max_of(g), b = TWO ? Bits<T>::max_of(v) : 0u;
+    if constexpr (sizeof(T) == 2) {
+        a |= b << 16;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) a = __vmaxu2(a, __shfl_xor_sync(0xffffffffu, a, o));
+        return make_uint2(a & 0xFFFFu, a >> 16);
+    } else {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+            a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+            if (TWO) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+        }
+        return make_uint2(a, b);
+    }
 }
 
-// MODE: 0 keep and restore nothing else (x -> q, scales), 1 ungated, 2 gated; KEEP: write q and scales
+// Infinity or NaN in the block: NaN in their place, and the largest of the others.  Rare; the lanes of a block come here together.
+__device__ __forceinline__ float finite_max(float2 (&x)[4]) {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (!(fabsf(x[e].x) <= 3.402823466e38f)) x[e].x = __int_as_float(0x7FC00000);
+        if (!(fabsf(x[e].y) <= 3.402823466e38f)) x[e].y = __int_as_float(0x7FC00000);
+        m = fmaxf(m, fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
+    }
+    const uint32_t mask = 0xFFFFu << (threadIdx.x & 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, o));
+    return m;
+}
+
+// e4m3 values and scale of a block whose largest bits are `top`
+template <typename T>
+__device__ __forceinline__ uint2 keep(float2 (&x)[4], uint32_t top, float* scale) {
+    const float amax = top >= Bits<T>::kInf ? finite_max(x) : Bits<T>::value(top);
+    const float2 s = exact_pow2_scale(amax), inv = make_float2(s.y, s.y);
+    *scale = s.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __fmul2_rn(x[e], inv);
+    return make_uint2(pack_e4m3x4(x[0].x, x[0].y, x[1].x, x[1].y), pack_e4m3x4(x[2].x, x[2].y, x[3].x, x[3].y));
+}
+
+// Row and octet of a flat item, and of the one a stride further without another division
+struct Place {
+    uint32_t row, col;
+    __device__ Place(uint32_t item, uint32_t octets) : row(item / octets), col(item - row * octets) {}
+    __device__ void advance(const Place& by, uint32_t octets) {
+        row += by.row;
+        col += by.col;
+        if (col >= octets) {
+            col -= octets;
+            ++row;
+        }
+    }
+};
+
+// MODE: 0 keep and nothing else (x -> q, scales), 1 ungated, 2 gated; KEEP: write q and scales
 template <typename T, int MODE, bool KEEP>
 __global__ void __launch_bounds__(kThreads)
 gate_kernel(const T* __restrict__ up, T* __restrict__ h, uint2* __restrict__ q, float* __restrict__ scales, uint32_t items, uint32_t octets,
@@ -59,49 +135,51 @@ gate_kernel(const T* __restrict__ up, T* __restrict__ h, uint2* __restrict__ q, 
     // items: octets of the activation in all rows; octets: of one row.  gate_at: 0 = the gate is the first half, 1 the second
     const uint32_t stride = gridDim.x * kThreads;
     const uint32_t width = MODE == 2 ? 2 * octets : octets;          // octets of an input row
+    const uint32_t to_gate = MODE == 2 ? gate_at * octets : 0, to_value = (gate_at ^ 1) * octets;
+    const Place by(stride, octets);
+    Place place(blockIdx.x * kThreads + threadIdx.x, octets);
     // every lane of a warp walks the same number of rounds: the shuffles name all of them
     for (uint32_t base = blockIdx.x * kThreads + threadIdx.x; base - (threadIdx.x & 31) < items; base += kUnroll * stride) {
         Octet<T> rg[kUnroll], rv[kUnroll];
-        uint32_t at[kUnroll];
         int64_t in[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            at[u] = base + u * stride;
             rg[u].clear();
             rv[u].clear();
-            in[u] = 0;
-            if (at[u] < items) {
-                const uint32_t row = at[u] / octets;
-                in[u] = static_cast<int64_t>(row) * width + (at[u] - row * octets);
-                rg[u].load(up + (in[u] + (MODE == 2 ? gate_at * octets : 0)) * 8);
-                if (MODE == 2) rv[u].load(up + (in[u] + (gate_at ^ 1) * octets) * 8);
+            in[u] = static_cast<int64_t>(place.row) * width + place.col;
+            if (base + u * stride < items) {
+                rg[u].load(up + (in[u] + to_gate) * 8);
+                if (MODE == 2) rv[u].load(up + (in[u] + to_value) * 8);
             }
+            place.advance(by, octets);
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            float g[8], v[8], o[8];
-            rg[u].unpack(g);
-            if (MODE == 2) rv[u].unpack(v);
+            const bool live = base + u * stride < items;
+            float2 g[4], v[4];
+            rg[u].unpack2(g);
+            if (MODE == 2) rv[u].unpack2(v);
             if (MODE != 0) {
+                float2 o[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    o[e] = g[e] * sigmoid<T>(g[e]);
-                    if (MODE == 2) o[e] *= v[e];
+                for (int e = 0; e < 4; ++e) {
+                    o[e] = __fmul2_rn(g[e], make_float2(sigmoid<T>(g[e].x), sigmoid<T>(g[e].y)));
+                    if (MODE == 2) o[e] = __fmul2_rn(o[e], v[e]);
                 }
+                if (live) Octet<T>::store2(h + static_cast<int64_t>(base + u * stride) * 8, o);
             }
-            const bool live = at[u] < items;
-            if (MODE != 0 && live) Octet<T>::store(h + static_cast<int64_t>(at[u]) * 8, o);
             if (KEEP) {
                 float s;
-                const int64_t og = in[u] + (MODE == 2 ? gate_at * octets : 0);
-                const uint2 wg = keep(g, &s);
+                const uint2 top = block_max<T, MODE == 2>(rg[u], rv[u]);
+                const int64_t og = in[u] + to_gate;
+                const uint2 wg = keep<T>(g, top.x, &s);
                 if (live) {
                     q[og] = wg;
                     if ((threadIdx.x & 15) == 0) scales[og >> 4] = s;
                 }
                 if (MODE == 2) {
-                    const int64_t ov = in[u] + (gate_at ^ 1) * octets;
-                    const uint2 wv = keep(v, &s);
+                    const int64_t ov = in[u] + to_value;
+                    const uint2 wv = keep<T>(v, top.y, &s);
                     if (live) {
                         q[ov] = wv;
                         if ((threadIdx.x & 15) == 0) scales[ov >> 4] = s;
@@ -121,67 +199,75 @@ gate_bwd_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, c
     chain_wait();
     const uint32_t stride = gridDim.x * kThreads;
     const uint32_t width = MODE == 2 ? 2 * octets : octets;
+    const uint32_t to_gate = MODE == 2 ? gate_at * octets : 0, to_value = (gate_at ^ 1) * octets;
+    const Place by(stride, octets);
+    Place place(blockIdx.x * kThreads + threadIdx.x, octets);
     for (uint32_t base = blockIdx.x * kThreads + threadIdx.x; base < items; base += kUnroll * stride) {
         uint2 qg[kUnroll], qv[kUnroll];
         float sg[kUnroll], sv[kUnroll];
         Octet<T> rd[kUnroll];
-        uint32_t at[kUnroll];
         int64_t in[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            at[u] = base + u * stride;
-            if (at[u] < items) {
-                const uint32_t row = at[u] / octets;
-                in[u] = static_cast<int64_t>(row) * width + (at[u] - row * octets);
-                const int64_t ig = in[u] + (MODE == 2 ? gate_at * octets : 0), iv = in[u] + (gate_at ^ 1) * octets;
+            in[u] = static_cast<int64_t>(place.row) * width + place.col;
+            if (base + u * stride < items) {
+                const int64_t ig = in[u] + to_gate, iv = in[u] + to_value;
                 qg[u] = __ldcs(q + ig);
                 sg[u] = __ldg(scales + (ig >> 4));
                 if (MODE == 2) {
                     qv[u] = __ldcs(q + iv);
                     sv[u] = __ldg(scales + (iv >> 4));
                 }
-                if (MODE != 0) rd[u].load(dh + static_cast<int64_t>(at[u]) * 8);
+                if (MODE != 0) rd[u].load(dh + static_cast<int64_t>(base + u * stride) * 8);
             }
+            place.advance(by, octets);
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            if (at[u] >= items) continue;
-            float g[8], v[8], d[8], o[8], dv[8];
+            if (base + u * stride >= items) continue;
+            float2 g[4], v[4], d[4], o[4];
             unpack_e4m3x8(qg[u], g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] *= sg[u];
-            const int64_t ig = (in[u] + (MODE == 2 ? gate_at * octets : 0)) * 8;
+            for (int e = 0; e < 4; ++e) g[e] = __fmul2_rn(g[e], make_float2(sg[u], sg[u]));
+            const int64_t ig = (in[u] + to_gate) * 8;
             if (MODE == 0) {
-                Octet<T>::store(dup + ig, g);
+                Octet<T>::store2(dup + ig, g);
                 continue;
             }
-            if (MODE == 2) unpack_e4m3x8(qv[u], v);
-            rd[u].unpack(d);
+            if (MODE == 2) {
+                unpack_e4m3x8(qv[u], v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float sig = sigmoid<T>(g[e]);
-                const float silu = g[e] * sig;
-                const float slope = sig * fmaf(g[e], 1.0f - sig, 1.0f);
+                for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(v[e], make_float2(sv[u], sv[u]));
+            }
+            rd[u].unpack2(d);
+            const float2 one = make_float2(1.f, 1.f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 sig = make_float2(sigmoid<T>(g[e].x), sigmoid<T>(g[e].y));
+                const float2 silu = __fmul2_rn(g[e], sig);
+                // sig (1 + g (1 - sig)) = sig + silu (1 - sig)
+                const float2 slope = __ffma2_rn(silu, __fadd2_rn(one, make_float2(-sig.x, -sig.y)), sig);
                 if (MODE == 2) {
-                    const float val = v[e] * sv[u];
-                    o[e] = silu * val;
-                    dv[e] = d[e] * silu;
-                    d[e] = d[e] * val * slope;
+                    o[e] = __fmul2_rn(silu, v[e]);
+                    v[e] = __fmul2_rn(d[e], v[e]);
+                    g[e] = __fmul2_rn(d[e], silu);
+                    d[e] = __fmul2_rn(v[e], slope);
                 } else {
                     o[e] = silu;
-                    d[e] *= slope;
+                    d[e] = __fmul2_rn(d[e], slope);
                 }
             }
-            Octet<T>::store(dup + ig, d);
-            if (MODE == 2) Octet<T>::store(dup + (in[u] + (gate_at ^ 1) * octets) * 8, dv);
-            if (h != nullptr) Octet<T>::store(h + static_cast<int64_t>(at[u]) * 8, o);
+            Octet<T>::store2(dup + ig, d);
+            if (MODE == 2) Octet<T>::store2(dup + (in[u] + to_value) * 8, g);
+            if (h != nullptr) Octet<T>::store2(h + static_cast<int64_t>(base + u * stride) * 8, o);
         }
     }
 }
 
-unsigned grid_of(int64_t items) {
+// CTAs an SM at most: forward 16 (8: 93.4, 16: 92.7, 64: 96.1 us at 32768 x 2048, gated), backward 64 (8: 118.6, 16: 112.3, 64: 105.5)
+unsigned grid_of(int64_t items, int per_sm) {
     const int64_t ctas = (items + kThreads * kUnroll - 1) / (kThreads * kUnroll);
-    const int64_t cap = static_cast<int64_t>(device_info().sm_count) * 16;
+    const int64_t cap = static_cast<int64_t>(device_info().sm_count) * per_sm;
     return static_cast<unsigned>(ctas > cap ? cap : ctas);
 }
 
@@ -195,7 +281,7 @@ int run_gate(const void* up, void* h, void* q, float* scales, int64_t rows, int3
     const int64_t chunk = kMaxItems / octets;
     for (int64_t r = 0; r < rows; r += chunk) {
         const int64_t n = rows - r < chunk ? rows - r : chunk;
-        launch_chained(gate_kernel<T, MODE, KEEP>, grid_of(n * octets), kThreads, 0, st, static_cast<const T*>(up) + r * width * 8,
+        launch_chained(gate_kernel<T, MODE, KEEP>, grid_of(n * octets, 16), kThreads, 0, st, static_cast<const T*>(up) + r * width * 8,
                        h == nullptr ? nullptr : static_cast<T*>(h) + r * hidden, KEEP ? static_cast<uint2*>(q) + r * width : nullptr,
                        KEEP ? scales + r * width / 16 : nullptr, static_cast<uint32_t>(n * octets), static_cast<uint32_t>(octets), gate_at);
         count_launch();
@@ -212,7 +298,7 @@ int run_gate_bwd(const void* q, const float* scales, const void* dh, void* dup, 
     const int64_t chunk = kMaxItems / octets;
     for (int64_t r = 0; r < rows; r += chunk) {
         const int64_t n = rows - r < chunk ? rows - r : chunk;
-        launch_chained(gate_bwd_kernel<T, MODE>, grid_of(n * octets), kThreads, 0, st, static_cast<const uint2*>(q) + r * width,
+        launch_chained(gate_bwd_kernel<T, MODE>, grid_of(n * octets, 64), kThreads, 0, st, static_cast<const uint2*>(q) + r * width,
                        scales + r * width / 16, MODE == 0 ? nullptr : static_cast<const T*>(dh) + r * hidden,
                        static_cast<T*>(dup) + r * width * 8, h == nullptr ? nullptr : static_cast<T*>(h) + r * hidden,
                        static_cast<uint32_t>(n * octets), static_cast<uint32_t>(octets), gate_at);

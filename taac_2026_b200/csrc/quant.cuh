@@ -42,14 +42,12 @@ __device__ __forceinline__ float2 exact_pow2_scale(float amax) {
 }
 
 // eight e4m3 bytes -> floats
-__device__ __forceinline__ void unpack_e4m3x8(uint2 q, float (&f)[8]) {
+__device__ __forceinline__ void unpack_e4m3x8(uint2 q, float2 (&f)[4]) {
     const uint32_t w[2] = {q.x, q.y};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        f[2 * i] = v.x;
-        f[2 * i + 1] = v.y;
+        f[i] = __half22float2(*reinterpret_cast<const __half2*>(&h));
     }
 }
 
