@@ -20,7 +20,8 @@
 //
 // Distribution.  Row tiles go round robin over the pairs.  The tiles of the weight gradients of uneven experts differ in
 // length: most go round robin as well, the rest is cut into shares that even the pairs out (see Line), and a tile that two or
-// more pairs share leaves fp32 partial tiles in a workspace, which `ragged_join_kernel` adds in the order of the pairs.
+// more pairs share leaves fp32 partial tiles in a workspace, which `ragged_join_kernel` adds in the order of the pairs.  The bias
+// gradient comes with the weight gradient: four more warps add the rows of dy that lie in shared memory.
 //
 // Every wait on an mbarrier is bounded; a wait that gives up raises the status word and all roles drain through the final barrier.
 #include "ragged.cuh"
@@ -42,6 +43,7 @@ constexpr uint32_t kChunkBytes = 64 * 128;                // MN-major: 64 contra
 constexpr int kMaxStages = 6;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + kEpiWarps * 32;
+constexpr int kSumWarps = 4;                              // weights with a bias gradient: warps that add the rows of dy
 constexpr uint32_t kBoxBytes = 32 * 128;                  // an epilogue warp's staging box: 32 rows x 64 columns
 constexpr uint32_t kTmemCols = 512;
 constexpr int kSnap = 4;
@@ -286,13 +288,13 @@ __device__ __forceinline__ void clear_tail(uint8_t* stage, int valid, int lane) 
 }
 
 template <typename T, int MODE, bool RES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads + (MODE == kWeights ? kSumWarps * 32 : 0), 1)
 ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                    const __grid_constant__ CUtensorMap tmap_o, const RaggedArgs g) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_bar[kMaxStages];     // used in the leader only
     __shared__ uint64_t empty_bar[kMaxStages];
-    __shared__ uint64_t tail_bar[kMaxStages];     // weights, the other CTA: its own loads of an expert's last block
+    __shared__ uint64_t own_bar[kMaxStages];      // weights, the other CTA: its own loads
     __shared__ uint64_t tmem_full[2];
     __shared__ uint64_t tmem_empty[2];            // used in the leader only
     __shared__ uint32_t tmem_base_slot;
@@ -311,8 +313,8 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     if (threadIdx.x == 0) {
         for (int s = 0; s < g.stages; ++s) {
             mbar_init(&full_bar[s], MODE == kWeights ? 2 : 1);
-            mbar_init(&empty_bar[s], 1);
-            mbar_init(&tail_bar[s], 1);
+            mbar_init(&empty_bar[s], MODE == kWeights && g.db != nullptr ? 1 + kSumWarps : 1);
+            mbar_init(&own_bar[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tmem_full[b], 1);
@@ -359,23 +361,14 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                         const int64_t row = j.m0 + static_cast<int64_t>(b) * kBlock;
                         const int32_t y = static_cast<int32_t>(row);
                         const int32_t xa = (j.a0 + static_cast<int>(rank) * 128) * 2, xb = (j.b0 + static_cast<int>(rank) * 128) * 2;
-                        if (row + kBlock > j.end && rank != 0) {     // this CTA's warp 1 clears the rows behind the end and then tells the leader
-                            mbar_expect_tx(&tail_bar[s], kStageBytes);
-                            tma_load_2d(dst, &tmap_a, xa, y, &tail_bar[s]);
-                            tma_load_2d(dst + kChunkBytes, &tmap_a, xa + 128, y, &tail_bar[s]);
-                            tma_load_2d(dst + 2 * kChunkBytes, &tmap_b, xb, y, &tail_bar[s]);
-                            tma_load_2d(dst + 3 * kChunkBytes, &tmap_b, xb + 128, y, &tail_bar[s]);
-                        } else {
-                            if (rank == 0) {
-                                const bool tail = row + kBlock > j.end;
-                                mbar_expect_tx(&full_bar[s], tail ? kStageBytes : 2 * kStageBytes);
-                                if (!tail) mbar_arrive(&full_bar[s]);
-                            }
-                            tma_load_2d_pair(dst, &tmap_a, xa, y, &full_bar[s]);
-                            tma_load_2d_pair(dst + kChunkBytes, &tmap_a, xa + 128, y, &full_bar[s]);
-                            tma_load_2d_pair(dst + 2 * kChunkBytes, &tmap_b, xb, y, &full_bar[s]);
-                            tma_load_2d_pair(dst + 3 * kChunkBytes, &tmap_b, xb + 128, y, &full_bar[s]);
-                        }
+                        // each CTA's loads count in a barrier of its own, for the warps that add rows; the other CTA's warp 1 tells
+                        // the leader when its half is there
+                        uint64_t* bar = rank == 0 ? &full_bar[s] : &own_bar[s];
+                        mbar_expect_tx(bar, kStageBytes);
+                        tma_load_2d(dst, &tmap_a, xa, y, bar);
+                        tma_load_2d(dst + kChunkBytes, &tmap_a, xa + 128, y, bar);
+                        tma_load_2d(dst + 2 * kChunkBytes, &tmap_b, xb, y, bar);
+                        tma_load_2d(dst + 3 * kChunkBytes, &tmap_b, xb + 128, y, bar);
                     } else {
                         if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);   // the bytes of both CTAs
                         tma_load_2d_pair(dst, &tmap_a, b * 128, static_cast<int32_t>(j.m0) + static_cast<int>(rank) * 128, &full_bar[s]);
@@ -424,7 +417,7 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                         const int64_t valid = j.end - (j.m0 + static_cast<int64_t>(b) * kBlock);
                         if (valid < kBlock) {
                             depth = tail_depth(static_cast<int>(valid));
-                            asm volatile("fence.acq_rel.cluster;" ::: "memory");      // the other CTA has cleared its half
+                            asm volatile("fence.acq_rel.cluster;" ::: "memory");      // the other CTA has cleared its last rows
                             clear_tail(ring + static_cast<size_t>(s) * kStageBytes, static_cast<int>(valid), lane);
                         }
                     }
@@ -454,26 +447,91 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                 if (g.status != nullptr) atomicExch(g.status, 1);
             }
         } else if (MODE == kWeights) {
-            // ------------------------------------------------------------ the other CTA's last blocks
-            uint32_t s = 0, tail_ph = 0;
+            // ------------------------------------------------------------ the other CTA's half of a stage is there (and its last rows cleared)
+            uint32_t s = 0, ph = 0;
             bool ok = true;
             while (ok && walk.next(j)) {
                 for (int b = 0; b < j.blocks; ++b) {
+                    if (!mbar_wait_warp(&own_bar[s], ph)) { ok = false; break; }
                     const int64_t valid = j.end - (j.m0 + static_cast<int64_t>(b) * kBlock);
                     if (valid < kBlock) {
-                        if (!mbar_wait_warp(&tail_bar[s], (tail_ph >> s) & 1)) { ok = false; break; }
-                        tail_ph ^= 1u << s;
                         clear_tail(ring + static_cast<size_t>(s) * kStageBytes, static_cast<int>(valid), lane);
-                        if (lane == 0) mbar_arrive_leader_release(&full_bar[s]);
-                        __syncwarp();
+                        if (lane == 0) mbar_arrive_leader_release(&full_bar[s]);      // writes of this warp: a release at cluster scope, which takes a microsecond
+                    } else if (lane == 0) {
+                        mbar_arrive_leader(&full_bar[s]);
                     }
-                    if (++s == static_cast<uint32_t>(g.stages)) s = 0;
+                    __syncwarp();
+                    if (++s == static_cast<uint32_t>(g.stages)) {
+                        s = 0;
+                        ph ^= 1;
+                    }
                 }
             }
             if (!ok) {
                 s_abort = 1;
                 if (g.status != nullptr) atomicExch(g.status, 1);
             }
+        }
+    } else if (MODE == kWeights && warp >= 2 + kEpiWarps) {
+        // ---------------------------------------------------------------- bias gradient (both CTAs, own 128 rows of dw)
+        // The rows of dy pass through shared memory for the tiles of the first column anyway: a warp adds them for 32 of the
+        // CTA's columns of dy, a lane for eight of them and every eighth row (the order of the rows keeps the lanes of a phase in
+        // different banks), and the eight lanes of a column join at the end of the piece.  For the other tiles it only follows.
+        const int sw = warp - 2 - kEpiWarps;
+        const int sub = ((lane >> 2) & 1) << 2 | lane >> 3;              // this lane's row among eight
+        const int pc = (sw & 1) * 4 + (lane & 3);                        // its 16-byte piece of the chunk's 128 bytes
+        const uint8_t* chunk = ring + (sw >> 1) * kChunkBytes;
+        uint64_t* bar = rank == 0 ? full_bar : own_bar;
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        while (ok && walk.next(j)) {
+            const bool adds = j.b0 == 0;
+            float2 acc[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = make_float2(0.f, 0.f);
+            for (int b = 0; b < j.blocks; ++b) {
+                if (!mbar_wait_warp(&bar[s], ph)) { ok = false; break; }
+                if (adds) {
+                    const int64_t valid = j.end - (j.m0 + static_cast<int64_t>(b) * kBlock);
+                    const uint8_t* at = chunk + static_cast<size_t>(s) * kStageBytes;
+#pragma unroll
+                    for (int i = 0; i < kBlock / 8; ++i) {
+                        const int r = i * 8 + sub;
+                        if (r < valid) {
+                            float2 v[4];
+                            Vec16<T>::unpack2(*reinterpret_cast<const uint4*>(at + r * 128 + ((pc ^ (r & 7)) << 4)), v);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[e] = __fadd2_rn(acc[e], v[e]);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty_bar[s]);
+                if (++s == static_cast<uint32_t>(g.stages)) {
+                    s = 0;
+                    ph ^= 1;
+                }
+            }
+            if (!adds) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    acc[e].x += __shfl_xor_sync(0xffffffffu, acc[e].x, o);
+                    acc[e].y += __shfl_xor_sync(0xffffffffu, acc[e].y, o);
+                }
+            }
+            const int c = static_cast<int>(rank) * 128 + sw * 32 + (lane & 3) * 8;      // of the tile's 256
+            float* dst = j.slot >= 0 ? g.db_partial + (static_cast<int64_t>(pair) * 2 + j.slot) * kTile + c
+                                     : g.db + static_cast<int64_t>(j.e) * g.n + j.a0 + c;
+            if (lane < 4 && j.a0 + c < g.n) {
+                *reinterpret_cast<float4*>(dst) = make_float4(acc[0].x, acc[0].y, acc[1].x, acc[1].y);
+                *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[2].x, acc[2].y, acc[3].x, acc[3].y);
+            }
+        }
+        if (!ok) {
+            s_abort = 1;
+            if (g.status != nullptr) atomicExch(g.status, 1);
         }
     } else {
         // ---------------------------------------------------------------- epilogue (both CTAs, own 128 rows)
@@ -642,6 +700,16 @@ __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, in
     const int4 mine = __ldcg(g.pieces + 2 * blockIdx.x + 1);
     if (mine.x < 0) return;
     const int r = threadIdx.x;
+    if (blockIdx.y == 0 && g.db != nullptr && mine.z == 0 && mine.y + r < g.n) {
+        float sum = __ldcg(g.db_partial + (2 * static_cast<int64_t>(blockIdx.x) + 1) * kTile + r);
+        for (int k = blockIdx.x + 1; k < pairs; ++k) {
+            const int4 next = __ldcg(g.pieces + 2 * k);
+            if (next.x < 0) continue;
+            sum += __ldcg(g.db_partial + 2 * static_cast<int64_t>(k) * kTile + r);
+            if (next.w != 0) break;
+        }
+        g.db[static_cast<int64_t>(mine.x) * g.n + mine.y + r] = sum;
+    }
     const int row = mine.y + r, col = mine.z + blockIdx.y * 32;
     float4 sum[8];
     auto add = [&](int pair, int slot, bool first) {
@@ -671,7 +739,7 @@ __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, in
     }
 }
 
-// db[e] = sum of the expert's rows of dy, in two steps of fixed order.  Step one: CTA (x, y) adds the rows of chunk x, `chunk` rows
+// db[e] = sum of the expert's rows of dy where no weight gradient is wanted, in two steps of fixed order.  Step one: CTA (x, y) adds the rows of chunk x, `chunk` rows
 // of the matrix, for blockDim.x * 8 columns, and leaves a partial sum for every expert that has rows among them; that of
 // expert e stands in row x + e of the table, which no other pair of chunk and expert has, for both grow along the matrix.
 // Thread (tx, ty) takes eight columns of every blockDim.y-th row, eight loads in flight.  As many chunks as CTAs fit the chip:
@@ -772,7 +840,8 @@ int launch_pairs(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& 
         cudaFuncSetAttribute(ragged_pair_kernel<T, MODE, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
         attr_set[dev.index] = true;
     }
-    launch_chained(ragged_pair_kernel<T, MODE, RES>, 2 * pairs, kThreads, smem_of(g.stages, g.experts), st, a, b, o, g);
+    const int threads = kThreads + (MODE == kWeights && g.db != nullptr ? kSumWarps * 32 : 0);
+    launch_chained(ragged_pair_kernel<T, MODE, RES>, 2 * pairs, threads, smem_of(g.stages, g.experts), st, a, b, o, g);
     count_launch();
     return launch_status();
 }
@@ -828,7 +897,7 @@ int weights_of(const void* x, const void* dy, RaggedArgs g, cudaStream_t st) {
 }
 
 // floats of the workspace for shared tiles: their descriptions and the partial tiles
-int64_t share_floats(int64_t T) { return T >= kShareRows ? static_cast<int64_t>(pairs_here()) * (8 + 2 * kPartFloats) : 0; }
+int64_t share_floats(int64_t T) { return T >= kShareRows ? static_cast<int64_t>(pairs_here()) * (8 + 2 * kTile + 2 * kPartFloats) : 0; }
 
 // How the sum of the bias gradient's rows is laid over the chip: as many threads along the columns as there are octets (whole warps, at
 // most the CTA), the others along the rows; four CTAs an SM, at least 16 rows each
@@ -911,7 +980,7 @@ extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int3
     if (experts == 0) return TB200_OK;
     if ((dw == nullptr && db == nullptr) || (T > 0 && (dy == nullptr || offsets == nullptr || workspace == nullptr || (x == nullptr && dw != nullptr))))
         return TB200_ERR_NULL;
-    if (!aligned16(x) || !aligned16(dy) || !aligned16(dw) || !aligned16(workspace) || !aligned4(db) || !aligned4(offsets)) return TB200_ERR_ALIGN;
+    if (!aligned16(x) || !aligned16(dy) || !aligned16(dw) || !aligned16(workspace) || !aligned16(db) || !aligned4(offsets)) return TB200_ERR_ALIGN;
     if (!device_info().valid) return TB200_ERR_DEVICE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (T == 0) {
@@ -930,10 +999,13 @@ extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int3
     g.n = N;
     if (T >= kShareRows) {
         g.pieces = reinterpret_cast<int4*>(workspace);
-        g.partial = workspace + pairs_here() * 8;
+        g.db_partial = workspace + pairs_here() * 8;
+        g.partial = g.db_partial + pairs_here() * 2 * kTile;
     }
-    if (dw != nullptr) code = dtype == TB200_BF16 ? weights_of<__nv_bfloat16>(x, dy, g, st) : weights_of<__half>(x, dy, g, st);
-    if (code != TB200_OK || db == nullptr) return code;
+    if (dw != nullptr) {
+        g.db = db;
+        return dtype == TB200_BF16 ? weights_of<__nv_bfloat16>(x, dy, g, st) : weights_of<__half>(x, dy, g, st);
+    }
     float* part = workspace + share_floats(T);
     const BiasShape b = bias_shape(T, N);
     const dim3 grid(static_cast<unsigned>(b.chunks), b.columns), block(b.tx, 256 / b.tx);

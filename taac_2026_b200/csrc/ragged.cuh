@@ -15,7 +15,9 @@ struct RaggedArgs {
     const float* bias;          // [experts, cols] or NULL (rows)
     const void* residual;       // [T, cols] or NULL (rows)
     void* out;                  // [T, cols], or [experts, n, k] (weights)
+    float* db;                  // [experts, n] or NULL (weights)
     float* partial;             // [pairs][2] partial tiles, NULL: tiles are never shared (weights)
+    float* db_partial;          // [pairs][2][256] sums of the rows of those pieces
     int4* pieces;               // [pairs][2] what they are part of: expert (-1: nothing), first row and column of the tile, last piece?
     int32_t* status;
     int32_t experts, stages;

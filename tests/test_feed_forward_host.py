@@ -149,4 +149,4 @@ def test_ragged_entries(lib):
     assert wgrad(P(p), P(p), P(p), None, None, P(p), 2, 4, 64, 64, BF16, None, None) == ERR_NULL
     assert wgrad(P(p), P(p), P(p), P(p), None, None, 2, 4, 64, 64, BF16, None, None) == ERR_NULL
     assert wgrad(None, P(p), P(p), P(p), None, P(p), 2, 4, 64, 64, BF16, None, None) == ERR_NULL
-    assert wgrad(P(p), P(p), P(p), P(p), P(p + 2), P(p), 2, 4, 64, 64, BF16, None, None) == ERR_ALIGN
+    assert wgrad(P(p), P(p), P(p), P(p), P(p + 4), P(p), 2, 4, 64, 64, BF16, None, None) == ERR_ALIGN

@@ -77,8 +77,8 @@ def _check_grads(dx, dw, db, x, w, dy, ends):
         _within(dx[r], want, _half(dtype) * want.abs() + _steps(n) * (ge.abs() @ we.abs()) + _tiny(dtype))
         want = ge.T @ xe
         _within(dw[e], want, _half(dtype) * want.abs() + _steps(len(xe)) * (ge.abs().T @ xe.abs()) + _tiny(dtype))
-        if db is not None:      # fp32: 32 rows in order in a warp, 8 warps, then the pieces of 256 rows
-            _within(db[e], ge.sum(0), (40 + len(xe) / 256) * 2.0 ** -24 * ge.abs().sum(0))
+        if db is not None:      # fp32: every eighth row in order in a lane (in a thread of 1 to 8 without dw), then 3 + 74 or 8 + 74 partial sums
+            _within(db[e], ge.sum(0), (100 + len(xe) / 8) * 2.0 ** -24 * ge.abs().sum(0))
 
 
 SIZES = [
@@ -114,7 +114,8 @@ def test_backward(dtype, sizes, n, k):
     only = ops.ragged_linear_backward(x, w, off, dy, need_x=False)
     assert only[0] is None and only[2] is None and torch.equal(only[1], dw)
     only = ops.ragged_linear_backward(x, w, off, dy, need_weight=False, bias=True)
-    assert only[1] is None and torch.equal(only[0], dx) and torch.equal(only[2], db)
+    assert only[1] is None and torch.equal(only[0], dx)
+    _check_grads(only[0], dw, only[2], x, w, dy, ends)                       # a kernel of its own adds the rows then
 
 
 @pytest.mark.parametrize("dtype", TYPES)
