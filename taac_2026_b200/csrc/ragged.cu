@@ -19,8 +19,8 @@
 // A row tile that crosses its expert's end computes rows of the next expert for nothing and does not store them.
 //
 // Distribution.  Row tiles go round robin over the pairs.  The tiles of the weight gradients of uneven experts differ in
-// length: most go round robin as well, the rest is cut into shares that even the pairs out (see Line), and a tile that two or
-// more pairs share leaves fp32 partial tiles in a workspace, which `ragged_join_kernel` adds in the order of the pairs.  The bias
+// length: they go round robin as well, the long ones first, unless that would leave pairs idle for long; then the rest is cut into
+// shares that even the pairs out (see Line), and a tile that two or more pairs share leaves fp32 partial tiles in a workspace, which `ragged_join_kernel` adds in the order of the pairs.  The bias
 // gradient comes with the weight gradient: four more warps add the rows of dy that lie in shared memory.
 //
 // Every wait on an mbarrier is bounded; a wait that gives up raises the status word and all roles drain through the final barrier.
@@ -61,10 +61,10 @@ __device__ __forceinline__ int row_blocks(const int32_t* begin, int e) {
 
 // How the tiles of the weight gradients are shared out.  All experts have `tiles` tiles, each as long as its expert has blocks.  The
 // experts stand in a line, the long ones in front (but those whose tiles are longer than a pair's equal share at the end), and
-// their tiles one after the other.  The first `wave_tiles` of the line go round robin, so that the pairs are on the same few
-// experts at a time and read the same rows while these are in the L2; every pair stays within its equal share there.
-// What lies behind is cut so that all pairs end up with equal shares.  Measured at 16 experts of 2048 rows, 2048 x 2048: 359 us
-// with one contiguous share for every pair (rows of all experts are in use all the time), 238 so.
+// their tiles one after the other.  The first `wave_tiles` of the line, mostly all, go round robin, so that the pairs are on the
+// same few experts at a time and read the same rows while these are in the L2.  What lies behind is cut so that all pairs end
+// up with equal shares: what few long tiles need.  Measured at 16 experts of 2048 rows, 2048 x 2048: 359 us with one contiguous
+// share for every pair (rows of all experts are in use all the time), 218 round robin.
 struct Line {
     int32_t* begin;       // [experts + 1] first rows
     int32_t* pre;         // [experts + 1] blocks of one column of tiles before the i-th expert of the line
@@ -106,10 +106,10 @@ __device__ void make_line(const RaggedArgs& g, const Line& line, int tiles, int 
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const int64_t total = static_cast<int64_t>(sum) * tiles, share = total / pairs;
     // the line: a counting sort by length, kClasses steps up to a pair's share, the longest first and those beyond it last
-    const int64_t width = share / kClasses + 1;
+    const int width = static_cast<int>((share < INT32_MAX ? share : INT32_MAX) / kClasses) + 1;
     auto class_of = [&](int e) {
         const int nb = row_blocks(line.begin, e);
-        return nb > share ? kClasses : kClasses - 1 - static_cast<int>((nb - 1) / width);
+        return nb > share ? kClasses : kClasses - 1 - (nb - 1) / width;
     };
     for (int c = lane; c <= kClasses; c += 32) line.place[c] = 0;
     __syncwarp();
@@ -139,7 +139,27 @@ __device__ void make_line(const RaggedArgs& g, const Line& line, int tiles, int 
         __syncwarp();
     }
     prefix(line.pre, g.experts, lane, [&](int i) { return row_blocks(line.begin, line.order[i]); });
-    // as many rounds as leave every pair within its share: none of a round's tiles is longer than its first one and a class
+    // The line as whole tiles, round after round of the pairs, each as long as its first tile: good enough unless it takes half as long
+    // again as equal shares would, and some.  Pairs that are done early leave the others their bandwidth, and a cut costs
+    // its partial tiles: 16 experts of 2048 rows, 512 -> 2048 (4 rounds for 3.5) take 63 us in whole tiles and 72 cut, 9 of 7282 rows
+    // 115 and 134; one expert of 8192 rows (16 tiles) 56 and 35.
+    const int64_t rounds = (static_cast<int64_t>(g.experts) * tiles + pairs - 1) / pairs;
+    int64_t span = 0;
+    for (int64_t w = lane; w < rounds; w += 32) {
+        const int i = static_cast<int>(w * pairs / tiles);
+        span += line.pre[i + 1] - line.pre[i];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) span += __shfl_xor_sync(0xffffffffu, span, o);
+    if (shorter == g.experts && 2 * span <= 3 * share + 12 * kSnap) {
+        if (lane == 0) {
+            *line.wave_tiles = static_cast<int64_t>(g.experts) * tiles;
+            line.cut[0] = line.cut[1] = 0;
+        }
+        __syncwarp();
+        return;
+    }
+    // else as many rounds as leave every pair within its share: none of a round's tiles is longer than its first one and a class
     const int64_t fit = static_cast<int64_t>(shorter) * tiles / pairs;
     int64_t waves = 0, reached = 0;
     for (bool more = fit > 0; more;) {

@@ -32,19 +32,26 @@ struct RaggedArgs {
 // Where every expert's rows begin, by one warp; the offsets come from the kernel in front.  An offset outside [0, T] is moved to
 // the nearer end and one that lies before an earlier one counts as that one, so that no two experts share a row.
 __device__ __forceinline__ void first_rows(const RaggedArgs& g, int32_t* begin, int lane) {
+    constexpr int kAhead = 4;      // loads in flight
     int32_t top = 0;
-    for (int base = 0; base <= g.experts; base += 32) {
-        int32_t v = 0;
-        if (base + lane <= g.experts) v = __ldcg(g.offsets + base + lane);
-        v = v < 0 ? 0 : (v > g.T ? static_cast<int32_t>(g.T) : v);
+    for (int base = 0; base <= g.experts; base += 32 * kAhead) {
+        int32_t v[kAhead];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v = max(v, u);
+        for (int k = 0; k < kAhead; ++k) v[k] = base + 32 * k + lane <= g.experts ? __ldcg(g.offsets + base + 32 * k + lane) : 0;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int at = base + 32 * k;
+            if (at > g.experts) break;
+            int32_t m = v[k] < 0 ? 0 : (v[k] > g.T ? static_cast<int32_t>(g.T) : v[k]);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int32_t u = __shfl_up_sync(0xffffffffu, m, o);
+                if (lane >= o) m = max(m, u);
+            }
+            m = max(m, top);
+            if (at + lane <= g.experts) begin[at + lane] = m;
+            top = __shfl_sync(0xffffffffu, m, 31);
         }
-        v = max(v, top);
-        if (base + lane <= g.experts) begin[base + lane] = v;
-        top = __shfl_sync(0xffffffffu, v, 31);
     }
     __syncwarp();
 }
