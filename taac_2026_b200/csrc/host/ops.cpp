@@ -688,6 +688,13 @@ int32_t* status_at(const std::optional<Tensor>& status, const Tensor& beside, bo
     return ok ? status->data_ptr<int32_t>() : nullptr;
 }
 
+// whether the bytes of two dense tensors overlap
+bool overlap(const Tensor& a, const Tensor& b) {
+    const auto* p = static_cast<const char*>(a.data_ptr());
+    const auto* q = static_cast<const char*>(b.data_ptr());
+    return a.numel() > 0 && b.numel() > 0 && p < q + b.nbytes() && q < p + a.nbytes();
+}
+
 // ragged_linear(x, weight, offsets, bias or None, silu, residual or None, out or None, status or None)
 PyObject* py_ragged_linear(PyObject*, PyObject* const* args, Py_ssize_t) {
     HANDLE_TH_ERRORS
@@ -705,6 +712,12 @@ PyObject* py_ragged_linear(PyObject*, PyObject* const* args, Py_ssize_t) {
     if (bias.has_value() && (!plain(*bias, at::kFloat, x) || bias->dim() != 2 || bias->size(0) != r.experts || bias->size(1) != r.n)) Py_RETURN_NONE;
     for (const auto* t : {&residual, &into})
         if (t->has_value() && (!plain(**t, x.scalar_type(), x) || (*t)->dim() != 2 || (*t)->size(0) != r.rows || (*t)->size(1) != r.n)) Py_RETURN_NONE;
+    if (into.has_value()) {   // it may be the residual, but shares no memory with the other operands
+        for (const Tensor* t : {&x, &w, &off})
+            if (overlap(*into, *t)) Py_RETURN_NONE;
+        if (bias.has_value() && overlap(*into, *bias)) Py_RETURN_NONE;
+        if (residual.has_value() && residual->data_ptr() != into->data_ptr() && overlap(*into, *residual)) Py_RETURN_NONE;
+    }
     bool ok = true;
     int32_t* word = status_at(status, x, ok);
     if (!ok) Py_RETURN_NONE;

@@ -1769,6 +1769,13 @@ def _ragged_operands(name: str, rows: torch.Tensor, weight: torch.Tensor, offset
         raise ValueError(f"{name} needs rows and weight of one dtype, got {rows.dtype} and {weight.dtype}")
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor | None) -> bool:
+    """Whether the bytes of two contiguous tensors overlap."""
+    if b is None or not a.numel() or not b.numel():
+        return False
+    return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
 def _raise_incomplete(name: str, check: bool, status: torch.Tensor | None) -> None:
     if check and int(status.item()) != 0:
         raise RuntimeError(f"cuda {name}: a bounded wait inside the kernel gave up; the output is incomplete")
@@ -1781,7 +1788,7 @@ def ragged_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, 
     expert e: linear layers grouped by expert, with sizes that only the device knows (tcgen05, fp32 accumulation).
 
     x: [T, K] with the rows sorted by expert; weight: [E, N, K]; offsets: int32 [E + 1] on the device, not decreasing (one
-    that is counts as the largest before it, and all are held inside [0, T]); bias: [E, N] (any float dtype; used as fp32);
+    that does counts as the largest before it, and all are held inside [0, T]); bias: [E, N] (any float dtype; used as fp32);
     residual / out: [T, N]; ``out`` may be ``residual``.  fp16 or bf16; N and K are multiples of 8.  Rows of no expert are
     zero in a fresh result and left as they are in ``out``.
 
@@ -1792,7 +1799,7 @@ def ragged_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, 
         if silu or out is not None:
             raise RuntimeError("cuda ragged_linear is forward-only with silu or out: use silu_gate(gated=False) behind it for training")
         _ragged_operands("ragged_linear", x, weight, offsets, 2)
-        return _RaggedLinearFunction.apply(x, weight, offsets, bias, residual, bool(checkpoint))
+        return _RaggedLinearFunction.apply(x, weight, offsets, bias, residual, bool(checkpoint), check, status)
     if _TIMING is None and not check:
         fast = _host.ragged_linear(x, weight, offsets, bias, silu, residual, out, status)
         if fast is not None:
@@ -1812,6 +1819,9 @@ def ragged_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, 
     x, weight = _aligned(x), _aligned(weight)
     res = None if residual is None else _aligned(residual)
     target = torch.empty(rows, n, dtype=x.dtype, device=x.device) if out is None else out
+    if out is not None and (any(_overlap(out, t) for t in (x, weight, bias32, offsets))
+                            or (_overlap(out, res) and res.data_ptr() != out.data_ptr())):
+        raise ValueError("ragged_linear: out may be residual, but shares no memory with the other operands")
     status = _status_word(check, status, x.device)
     with torch.cuda.device(x.device), _timed("ragged_linear", experts=experts, m=rows, n=n, k=k, silu=bool(silu)):
         code = _lib.load().tb200_ragged_gemm(_ptr(x), _ptr(weight), _ptr(offsets.contiguous()), _ptr(bias32), _ptr(res), _ptr(target), experts, rows,
@@ -1870,7 +1880,7 @@ def ragged_linear_backward(x: torch.Tensor, weight: torch.Tensor, offsets: torch
 
 class _RaggedLinearFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, offsets, bias, residual, checkpoint):
+    def forward(ctx, x, weight, offsets, bias, residual, checkpoint, check, status):
         kept = scales = None
         if weight.requires_grad:
             kept, scales = checkpoint_activation(x) if checkpoint else (x, None)
@@ -1878,16 +1888,16 @@ class _RaggedLinearFunction(torch.autograd.Function):
         ctx.rows = x.shape
         ctx.bias_dtype = None if bias is None else bias.dtype
         with torch.no_grad():
-            return ragged_linear(x, weight, offsets, bias, residual=residual)
+            return ragged_linear(x, weight, offsets, bias, residual=residual, check=check, status=status)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
         kept, scales, weight, offsets = ctx.saved_tensors
-        need_x, need_w, _o, need_b, need_r, _c = ctx.needs_input_grad
+        need_x, need_w, _o, need_b, need_r = ctx.needs_input_grad[:5]
         x = kept if kept is not None else grad_out.new_empty(1).expand(ctx.rows)     # its shape alone is read
         dx, dw, db = ragged_linear_backward(x, weight, offsets, grad_out, scales=scales, bias=need_b, need_x=need_x, need_weight=need_w)
-        return dx, dw, None, None if db is None else db.to(ctx.bias_dtype), grad_out if need_r else None, None
+        return dx, dw, None, None if db is None else db.to(ctx.bias_dtype), grad_out if need_r else None, None, None, None
 
 
 def ffn_fp8_static_capacity() -> int:

@@ -259,6 +259,14 @@ def test_empty_and_refused():
         ops.ragged_linear(x, w, off, residual=dy.float())
     with pytest.raises(RuntimeError, match="same device"):
         ops.ragged_linear(x, w, off.cpu())
+    for taken in (x, w[0, :8]):                          # N = K = 64: they would fit
+        with pytest.raises(ValueError, match="shares no memory"):
+            ops.ragged_linear(x, w, off, out=taken)
+    long = torch.zeros(16, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="shares no memory"):
+        ops.ragged_linear(x, w, off, residual=long[:8], out=long[4:12])
+    with pytest.raises(ValueError, match="out must be contiguous"):
+        ops.ragged_linear(x, w, off, out=torch.zeros(8, 128, device="cuda", dtype=torch.bfloat16)[:, :64])
 
 
 @pytest.mark.parametrize("experts", [200, 1500])
@@ -290,3 +298,129 @@ def test_first_call_of_a_thread():
     thread.join()
     torch.cuda.synchronize()
     assert got and torch.equal(got[0], want)
+
+
+def test_offsets_past_32_bits():
+    """2.2 * 10^9 outputs: the last expert's rows stand behind 2^32 bytes and 2^31 elements."""
+    rows, n, k = 540_000, 4096, 64
+    x = torch.zeros(rows, k, device="cuda", dtype=torch.bfloat16)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x[-300:] = torch.randn(300, k, generator=g, device="cuda").bfloat16()
+    w = torch.randn(2, n, k, generator=g, device="cuda").bfloat16()
+    ends = [0, rows - 200, rows]
+    off = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    out = ops.ragged_linear(x, w, off, check=True)
+    for e, r in ((0, slice(rows - 300, rows - 200)), (1, slice(rows - 200, rows))):
+        want = x[r].double() @ w[e].double().T
+        _within(out[r], want, _half(torch.bfloat16) * want.abs() + _steps(k) * (x[r].double().abs() @ w[e].double().abs().T) + 1e-9)
+    assert bool((out[:1000] == 0).all())
+    dx, dw, db = ops.ragged_linear_backward(x, w, off, out, bias=True, check=True)
+    r = slice(rows - 200, rows)
+    want = out[r].double() @ w[1].double()
+    _within(dx[r], want, _half(torch.bfloat16) * want.abs() + _steps(n) * (out[r].double().abs() @ w[1].double().abs()) + 1e-9)
+    want = out[r].double().T @ x[r].double()
+    _within(dw[1], want, _half(torch.bfloat16) * want.abs() + _steps(200) * (out[r].double().abs().T @ x[r].double().abs()) + 1e-9)
+
+
+@pytest.mark.parametrize("sizes", [[9000], [60, 60, 9000, 60], [1, 6000, 1, 1]])
+def test_tiles_shared_by_pairs(sizes):
+    """Few long tiles: their rows are cut between pairs and the partial sums joined, the bias gradient's among them."""
+    x, w, off, dy, bias, ends = _case(sizes, 520, 264, torch.bfloat16, 21)
+    dx, dw, db = ops.ragged_linear_backward(x, w, off, dy, bias=True, check=True)
+    _check_grads(dx, dw, db, x, w, dy, ends)
+    again = ops.ragged_linear_backward(x, w, off, dy, bias=True)
+    assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), again))
+
+
+@pytest.mark.parametrize("sizes,n,k", [([3, 1, 0, 2], 512, 1024), ([30, 20], 256, 2048), ([60, 64, 65], 128, 4096), ([1], 2048, 1024), ([17] * 70, 136, 520)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_rows(sizes, n, k, dtype):
+    """The kernel of few rows, with its contraction split over two and four CTAs and not at all, in both directions."""
+    x, w, off, dy, bias, ends = _case(sizes, n, k, dtype, 31)
+    _check_rows(ops.ragged_linear(x, w, off, bias, residual=dy, check=True), x, w, ends, bias, False, dy)
+    _check_rows(ops.ragged_linear(x, w, off, bias, silu=True, check=True), x, w, ends, bias, True)
+    dx, dw, db = ops.ragged_linear_backward(x, w, off, dy, bias=True, check=True)
+    _check_grads(dx, dw, db, x, w, dy, ends)
+
+
+def test_status_word_and_two_streams_at_once():
+    """Two calls at once on two streams, with a persistent status word each."""
+    cases = [_case([700, 300, 900], 520, 264, torch.bfloat16, s) for s in (41, 42)]
+    wants = [(ops.ragged_linear(x, w, off, bias), *ops.ragged_linear_backward(x, w, off, dy, bias=True)) for x, w, off, dy, bias, _e in cases]
+    words = [torch.zeros(1, dtype=torch.int32, device="cuda") for _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(3):
+        for i, (x, w, off, dy, bias, _e) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i] = (ops.ragged_linear(x, w, off, bias, status=words[i]), *ops.ragged_linear_backward(x, w, off, dy, bias=True, status=words[i]))
+    torch.cuda.synchronize()
+    assert all(int(v) == 0 for v in words)
+    for g, want in zip(got, wants):
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+def test_feed_forward_layer_as_a_training_step_uses_it():
+    """Residual norm, up projections by expert, gated activation kept in 8 bits, down projections, against the same chain in 64 bits
+    with the kept values in the backward pass's places: the loss's gradients of every weight."""
+    sizes, d, hidden = [40, 0, 100, 20], 256, 384
+    total_rows = sum(sizes)
+    g = torch.Generator(device="cuda").manual_seed(50)
+    make = lambda *s, k=1.0: torch.randn(*s, generator=g, device="cuda") * k  # noqa: E731
+    x, r = make(total_rows, d).bfloat16(), make(total_rows, d).bfloat16()
+    gamma = (1 + 0.1 * make(d)).bfloat16()
+    w_up, w_down = make(4, 2 * hidden, d, k=d ** -0.5).bfloat16(), make(4, d, hidden, k=hidden ** -0.5).bfloat16()
+    b_up, b_down = make(4, 2 * hidden, k=0.1), make(4, d, k=0.1)
+    dy = make(total_rows, d).bfloat16()
+    off = torch.tensor([0, 40, 40, 140, 160], dtype=torch.int32, device="cuda")
+    leaves = [t.clone().requires_grad_() for t in (x, r, gamma, w_up, b_up, w_down, b_down)]
+    t, n = ops.add_rms_norm(leaves[0], leaves[1], leaves[2])
+    u = ops.ragged_linear(n, leaves[3], off, leaves[4], checkpoint=True)
+    h = ops.silu_gate(u)
+    y = ops.ragged_linear(h, leaves[5], off, leaves[6], residual=t)
+    y.backward(dy)
+    assert torch.equal(leaves[0].grad, leaves[1].grad)
+
+    ref = [v.double().requires_grad_() for v in (x, r, gamma, w_up, b_up, w_down, b_down)]
+    td = ref[0] + ref[1]
+    nd = td * torch.rsqrt(td.pow(2).mean(-1, keepdim=True) + 1e-6) * ref[2]
+    index = torch.repeat_interleave(torch.arange(4, device="cuda"), torch.tensor(sizes, device="cuda"))
+    ud = torch.einsum("tk,tnk->tn", nd, ref[3][index]) + ref[4][index]
+    hd = torch.nn.functional.silu(ud[:, :hidden]) * ud[:, hidden:]
+    yd = torch.einsum("tk,tnk->tn", hd, ref[5][index]) + ref[6][index] + td
+    yd.backward(dy.double())
+    # roundings of bf16 (2^-8 each, four in a row forward, five back) and of e4m3 in the kept values (2^-4), as independent
+    # errors: in the 2-norm below 2^-4 / sqrt(3) * 1.5 for what passes the kept values, 10 * 2^-9 for the result
+    rel = lambda a, b: float((a.double() - b).norm() / b.norm())  # noqa: E731
+    assert rel(y.detach(), yd.detach()) <= 10 * 2.0 ** -9
+    for got, want in zip(leaves, ref):
+        assert got.grad is not None and rel(got.grad, want.grad) <= 1.5 * 2.0 ** -4 / 3 ** 0.5
+    # an expert without rows has zero gradients
+    for i in (3, 4, 5, 6):
+        assert bool((leaves[i].grad[1] == 0).all())
+
+
+def test_served_in_8_bits():
+    """The same layer as it is served: quantised residual norm -> e4m3 gated feed-forward layer with the sum as residual."""
+    g = torch.Generator(device="cuda").manual_seed(51)
+    x, r = (torch.randn(200, 512, generator=g, device="cuda").bfloat16() for _ in range(2))
+    gamma = torch.ones(512, device="cuda", dtype=torch.bfloat16)
+    w_up, w_down = (torch.randn(n, 512, generator=g, device="cuda") * 512 ** -0.5 for n in (1024, 512))
+    weights = ops.Fp8FfnWeights(w_up, w_down, gated=True)
+    total, q, scales = ops.add_rms_norm_quant(x, r, gamma)
+    h, sh = ops.fp8_gemm(q, scales, weights.w_up, weights.s_up, mode="swiglu", check=True)
+    got = ops.fp8_gemm(h, sh, weights.w_down, weights.s_down, mode="linear", residual=total, check=True)
+    n = _norm64(x.double() + r.double())
+    gate, value = (n @ w_up.double().T).chunk(2, -1)
+    want = (torch.nn.functional.silu(gate) * value) @ w_down.double().T
+    # Four e4m3 roundings, each at most 2^-4 of a value and as good as independent: 2^-4 / sqrt(3) = 0.036 in the 2-norm.  Rows and
+    # weights give gate and value 0.051 each, their product 0.072; with the hidden values' and the second weights' own it is 0.088.
+    # (Two such chains whose inputs differ by 2^-9 differ by a good part of that: a value that crosses a border of the
+    # first rounding moves hidden values over borders of the next, so they are not compared with each other.)
+    rel = float((got.double() - total.double() - want).norm() / want.norm())
+    assert rel <= 0.088
+
+
+def _norm64(t):
+    return t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + 1e-6)
