@@ -97,4 +97,17 @@ inline bool make_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The same matrices as chunks of 64 columns, for boxes of 64 rows x two chunks, which land chunk after chunk: the 128 columns of an
+// MN-major operand in one copy.  Whole chunks only: the last piece of a row would reach into the next.
+inline bool make_chunk_map(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t stack) {
+    const auto fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[4] = {128, rows, cols / 64, stack};
+    const cuuint64_t strides[3] = {2 * cols, 128, 2 * cols * rows};
+    const cuuint32_t box[4] = {128, 64, 2, 1};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, stack == 0 ? 3 : 4, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace tb200
