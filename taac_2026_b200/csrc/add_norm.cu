@@ -328,8 +328,10 @@ __global__ void __launch_bounds__(1024) add_norm_sum_kernel(const float* __restr
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int i = blockIdx.x * 32 + tx;
     float w = 0.f;
-    if (i < cols)
-        for (int p = ty; p < n_partials; p += 32) w += partial[static_cast<int64_t>(p) * cols + i];
+    if (i < cols) {
+#pragma unroll 8
+        for (int p = ty; p < n_partials; p += 32) w += __ldcg(partial + static_cast<int64_t>(p) * cols + i);
+    }
     sums[ty][tx] = w;
     __syncthreads();
     if (ty == 0 && i < cols) {
