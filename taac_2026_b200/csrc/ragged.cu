@@ -30,6 +30,7 @@
 namespace tb200 {
 void count_launch();
 int ragged_few(const void* rows, const void* w, const RaggedArgs& g, int32_t N, int32_t K, bool grads, bool bf16, cudaStream_t st);
+int ragged_few_weights(const void* x, const void* dy, const RaggedArgs& g, bool bf16, cudaStream_t st);
 
 namespace {
 
@@ -39,7 +40,6 @@ constexpr int kTile = 256;                                // of a pair, both way
 constexpr int kBlock = 64;                                // contracted per stage: 128 bytes of a 16-bit type, or 64 rows
 constexpr uint32_t kOperandBytes = 128 * 128;             // one CTA's half of an operand in a stage
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
-constexpr uint32_t kChunkBytes = 64 * 128;                // MN-major: 64 contraction rows x 128 bytes
 constexpr int kMaxStages = 6;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + kEpiWarps * 32;
@@ -294,31 +294,6 @@ struct Walk {
 };
 
 
-// 64 rows of 128 columns as an MN-major operand: two chunks of 64 columns, in one copy where the columns are whole chunks (16 experts of
-// 2048 rows, 2048 x 2048: 218 us in two copies, 199 in one)
-template <bool CHUNKED>
-__device__ __forceinline__ void load_rows(const CUtensorMap* map, uint8_t* dst, int32_t col, int32_t row, uint64_t* bar) {
-    if (CHUNKED) {
-        tma_load_3d(dst, map, 0, row, col / 64, bar);
-    } else {
-        tma_load_2d(dst, map, col * 2, row, bar);
-        tma_load_2d(dst + kChunkBytes, map, col * 2 + 128, row, bar);
-    }
-}
-
-// Contraction rows that an expert's last block is taken for: whole steps of 16, the depth of one MMA
-__device__ __forceinline__ int tail_depth(int valid) { return (valid + 15) & ~15; }
-// Sets the rows [valid, tail_depth(valid)) of a stage's four chunks to zero, by one warp: eight lanes a row
-__device__ __forceinline__ void clear_tail(uint8_t* stage, int valid, int lane) {
-    const int end = tail_depth(valid);
-    for (int r = valid + (lane >> 3); r < end; r += 4) {
-#pragma unroll
-        for (int chunk = 0; chunk < 4; ++chunk) *reinterpret_cast<uint4*>(stage + chunk * kChunkBytes + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-}
-
 // CHUNKED: the maps of MN-major operands have chunks of 64 columns (see make_chunk_map)
 template <typename T, int MODE, bool RES, bool CHUNKED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads + (MODE == kWeights ? kSumWarps * 32 : 0), 1)
@@ -356,6 +331,10 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         s_abort = 0;
         fence_mbar_init();
     }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tmap_a);
+        tma_prefetch_desc(&tmap_b);
+    }
     if (warp == 1) tmem_alloc_pair(&tmem_base_slot, kTmemCols);
     tc_fence_before_sync();
     __syncthreads();
@@ -379,8 +358,6 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer (both CTAs)
         if (lane == 0) {
-            tma_prefetch_desc(&tmap_a);
-            tma_prefetch_desc(&tmap_b);
             uint32_t s = 0, ph = 0;
             bool ok = true;
             while (ok && walk.next(j)) {
@@ -507,37 +484,18 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         }
     } else if (MODE == kWeights && warp >= 2 + kEpiWarps) {
         // ---------------------------------------------------------------- bias gradient (both CTAs, own 128 rows of dw)
-        // The rows of dy pass through shared memory for the tiles of the first column anyway: a warp adds them for 32 of the
-        // CTA's columns of dy, a lane for eight of them and every eighth row (the order of the rows keeps the lanes of a phase in
-        // different banks), and the eight lanes of a column join at the end of the piece.  For the other tiles it only follows.
+        // The rows of dy pass through shared memory for the tiles of the first column anyway; for the other tiles the warps only follow.
         const int sw = warp - 2 - kEpiWarps;
-        const int sub = ((lane >> 2) & 1) << 2 | lane >> 3;              // this lane's row among eight
-        const int pc = (sw & 1) * 4 + (lane & 3);                        // its 16-byte piece of the chunk's 128 bytes
-        const uint8_t* chunk = ring + (sw >> 1) * kChunkBytes;
+        RowSum<T> sum(sw, lane);
         uint64_t* bar = rank == 0 ? full_bar : own_bar;
         uint32_t s = 0, ph = 0;
         bool ok = true;
         while (ok && walk.next(j)) {
             const bool adds = j.b0 == 0;
-            float2 acc[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = make_float2(0.f, 0.f);
+            sum.clear();
             for (int b = 0; b < j.blocks; ++b) {
                 if (!mbar_wait_warp(&bar[s], ph)) { ok = false; break; }
-                if (adds) {
-                    const int64_t valid = j.end - (j.m0 + static_cast<int64_t>(b) * kBlock);
-                    const uint8_t* at = chunk + static_cast<size_t>(s) * kStageBytes;
-#pragma unroll
-                    for (int i = 0; i < kBlock / 8; ++i) {
-                        const int r = i * 8 + sub;
-                        if (r < valid) {
-                            float2 v[4];
-                            Vec16<T>::unpack2(*reinterpret_cast<const uint4*>(at + r * 128 + ((pc ^ (r & 7)) << 4)), v);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[e] = __fadd2_rn(acc[e], v[e]);
-                        }
-                    }
-                }
+                if (adds) sum.add(ring + static_cast<size_t>(s) * kStageBytes, j.end - (j.m0 + static_cast<int64_t>(b) * kBlock));
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty_bar[s]);
                 if (++s == static_cast<uint32_t>(g.stages)) {
@@ -546,21 +504,11 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                 }
             }
             if (!adds) continue;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) {
-                    acc[e].x += __shfl_xor_sync(0xffffffffu, acc[e].x, o);
-                    acc[e].y += __shfl_xor_sync(0xffffffffu, acc[e].y, o);
-                }
-            }
+            sum.join();
             const int c = static_cast<int>(rank) * 128 + sw * 32 + (lane & 3) * 8;      // of the tile's 256
-            float* dst = j.slot >= 0 ? g.db_partial + (static_cast<int64_t>(pair) * 2 + j.slot) * kTile + c
-                                     : g.db + static_cast<int64_t>(j.e) * g.n + j.a0 + c;
-            if (lane < 4 && j.a0 + c < g.n) {
-                *reinterpret_cast<float4*>(dst) = make_float4(acc[0].x, acc[0].y, acc[1].x, acc[1].y);
-                *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[2].x, acc[2].y, acc[3].x, acc[3].y);
-            }
+            if (lane < 4 && j.a0 + c < g.n)
+                sum.store(j.slot >= 0 ? g.db_partial + (static_cast<int64_t>(pair) * 2 + j.slot) * kTile + c
+                                      : g.db + static_cast<int64_t>(j.e) * g.n + j.a0 + c);
         }
         if (!ok) {
             s_abort = 1;
@@ -708,7 +656,7 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             g.pieces[2 * pair] = left0;
             g.pieces[2 * pair + 1] = left1;
         }
-        if (lane == 0) bulk_wait<0>();            // the last store must have left shared memory before the CTA ends
+        if (lane == 0) bulk_wait_read<0>();       // the last store must have left shared memory before the CTA ends
         if (!ok) {
             s_abort = 1;
             if (g.status != nullptr) atomicExch(g.status, 1);
@@ -917,8 +865,17 @@ int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bo
 // rows from which on a tile can be shared by pairs: with fewer, no expert has 2 kSnap blocks
 constexpr int64_t kShareRows = 2 * kSnap * kBlock;
 
+// Weight gradients go to the kernel of 128 x 128 tiles while the experts have up to kFewDepth rows each, or up to kFewLong where the 256 x
+// 256 tiles are no more than half of the pairs.  Measured, it / the pairs, with a bias gradient, in us: 16 experts of 128 rows, 512 ->
+// 2048, 15.8 / 20.4, of 512 29.1 / 30.0, of 1024 49.6 / 46.5; 256 of 128 rows, 512 -> 512, 48 / 61; 9 of 2048 rows, 512 -> 512 (36
+// tiles), 26 / 29; one of 1000, 512 -> 512 (4), 13 / 30; 3 of 5000, 1024 -> 512 (24), 65 / 41.
+constexpr int64_t kFewDepth = 768, kFewLong = 4096;
+
 template <typename T>
 int weights_of(const void* x, const void* dy, RaggedArgs g, cudaStream_t st) {
+    const int64_t tiles = static_cast<int64_t>(g.experts) * ((g.n + kTile - 1) / kTile) * ((g.cols + kTile - 1) / kTile);
+    if (g.T <= kFewDepth * g.experts || (2 * tiles <= pairs_here() && g.T <= kFewLong * g.experts))
+        return ragged_few_weights(x, dy, g, std::is_same<T, __nv_bfloat16>::value, st);
     CUtensorMap ta, tb, to;
     const uint64_t rows = static_cast<uint64_t>(g.T);
     const bool chunked = g.n % 64 == 0 && g.cols % 64 == 0;

@@ -82,6 +82,73 @@ __device__ __forceinline__ int expert_of(const int32_t* pre, int experts, int64_
     }
     return lo;
 }
+// ---- weight gradients: stages of 64 contraction rows, as chunks of 64 rows x 128 bytes (MN-major operands, 128-byte swizzle)
+constexpr uint32_t kChunkBytes = 64 * 128;
+
+// Contraction rows that an expert's last block is taken for: whole steps of 16, the depth of one MMA
+__device__ __forceinline__ int tail_depth(int valid) { return (valid + 15) & ~15; }
+// Sets the rows [valid, tail_depth(valid)) of a stage's four chunks to zero, by one warp: eight lanes a row
+__device__ __forceinline__ void clear_tail(uint8_t* stage, int valid, int lane) {
+    const int end = tail_depth(valid);
+    for (int r = valid + (lane >> 3); r < end; r += 4) {
+#pragma unroll
+        for (int chunk = 0; chunk < 4; ++chunk) *reinterpret_cast<uint4*>(stage + chunk * kChunkBytes + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+// 64 rows of 128 columns as an MN-major operand: two chunks of 64 columns, in one copy where the columns are whole chunks (16 experts of
+// 2048 rows, 2048 x 2048: 218 us in two copies, 194 in one)
+template <bool CHUNKED>
+__device__ __forceinline__ void load_rows(const CUtensorMap* map, uint8_t* dst, int32_t col, int32_t row, uint64_t* bar) {
+    if (CHUNKED) {
+        tma_load_3d(dst, map, 0, row, col / 64, bar);
+    } else {
+        tma_load_2d(dst, map, col * 2, row, bar);
+        tma_load_2d(dst + kChunkBytes, map, col * 2 + 128, row, bar);
+    }
+}
+// The bias gradient from the dy tiles in shared memory: one of four warps adds the rows for 32 of a tile's 128 columns, a lane for
+// eight of them and every eighth row (the order of the rows keeps the lanes of a phase in different banks).
+template <typename T>
+struct RowSum {
+    float2 acc[4];
+    int sub, piece;              // this lane's row among eight, and its 16-byte piece of the chunk's 128 bytes
+    uint32_t chunk;
+    __device__ RowSum(int warp, int lane) : sub(((lane >> 2) & 1) << 2 | lane >> 3), piece((warp & 1) * 4 + (lane & 3)), chunk((warp >> 1) * kChunkBytes) {}
+    __device__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = make_float2(0.f, 0.f);
+    }
+    __device__ void add(const uint8_t* stage, int64_t valid) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 8 + sub;
+            if (r < valid) {
+                float2 v[4];
+                Vec16<T>::unpack2(*reinterpret_cast<const uint4*>(stage + chunk + r * 128 + ((piece ^ (r & 7)) << 4)), v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = __fadd2_rn(acc[e], v[e]);
+            }
+        }
+    }
+    // the eight lanes of a column join; lanes 0 .. 3 hold the sums
+    __device__ void join() {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                acc[e].x += __shfl_xor_sync(0xffffffffu, acc[e].x, o);
+                acc[e].y += __shfl_xor_sync(0xffffffffu, acc[e].y, o);
+            }
+        }
+    }
+    __device__ void store(float* dst) const {
+        *reinterpret_cast<float4*>(dst) = make_float4(acc[0].x, acc[0].y, acc[1].x, acc[1].y);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[2].x, acc[2].y, acc[3].x, acc[3].y);
+    }
+};
+
 // silu(x) = x / (1 + exp(-x))
 __device__ __forceinline__ float silu(float x) { return x * __fdividef(1.0f, 1.0f + __expf(-x)); }
 

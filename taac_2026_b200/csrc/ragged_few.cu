@@ -26,7 +26,6 @@ constexpr int kThreads = 192;
 constexpr int kTile = 128;                      // output columns of a unit
 constexpr int kBlock = 64;
 constexpr uint32_t kWBytes = kTile * 128;
-constexpr uint32_t kChunkBytes = 64 * 128;
 constexpr uint32_t kRingBytes = 96 * 1024;      // two CTAs fit an SM
 constexpr int kMaxStages = 8;
 
@@ -282,6 +281,232 @@ ragged_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     }
 }
 
+// Weight gradients dw[e] = dy_e^T x_e in 128 x 128 tiles, a CTA each and round robin, two CTAs an SM: four times the tiles of the pair
+// kernel, each with a shorter start and a quarter of the epilogue, for layers whose experts have few rows or which have few tiles.
+// Both operands are MN-major, contracted over the expert's rows, the rows of the next expert in a last block cleared by the warp
+// that issues the MMAs; warps 2 to 5 turn the accumulator in shared memory, 32 columns at a time, so that four lanes write 64 bytes
+// of a row; warps 6 to 9 add the rows of dy for the bias gradient.
+constexpr int kSumWarps = 4;
+constexpr uint32_t kWeightStage = 4 * kChunkBytes;
+
+template <typename T, bool CHUNKED>
+__global__ void __launch_bounds__(kThreads + kSumWarps * 32, 2)
+ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __grid_constant__ CUtensorMap tmap_x, const RaggedArgs g) {
+    extern __shared__ uint8_t smem_raw[];
+    constexpr int kStages = kRingBytes / kWeightStage;
+    __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int s_abort;
+    __shared__ __align__(16) uint4 turn[4][32 * 4];             // a warp's 32 rows x 64 bytes
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    int32_t* begin = reinterpret_cast<int32_t*>(ring + kStages * kWeightStage);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], g.db != nullptr ? 1 + kSumWarps : 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], 4);
+        }
+        s_abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tmap_dy);
+        tma_prefetch_desc(&tmap_x);
+    }
+    if (warp == 1) {
+        tmem_alloc(&tmem_base_slot, 2 * kTile);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_base_slot;
+    chain_release();   // not before every CTA holds its tensor memory (see launch_chained)
+    chain_wait();
+    if (warp == 2) first_rows(g, begin, lane);
+    __syncthreads();
+
+    const int b_tiles = (g.cols + kTile - 1) / kTile, tiles = (g.n + kTile - 1) / kTile * b_tiles;
+    const int64_t units = static_cast<int64_t>(g.experts) * tiles;
+    int e, a0, b0, blocks;
+    int64_t first, rows;
+    auto decode = [&](int64_t u) {
+        e = static_cast<int>(u / tiles);
+        const int tile = static_cast<int>(u % tiles);
+        a0 = tile / b_tiles * kTile;
+        b0 = tile % b_tiles * kTile;
+        first = begin[e];
+        rows = begin[e + 1] - first;
+        blocks = static_cast<int>((rows + kBlock - 1) / kBlock);
+    };
+    uint32_t s = 0, ph = 0, buf = 0, aph = 0;
+    auto next_stage = [&]() {
+        if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+        }
+    };
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                decode(u);
+                for (int b = 0; b < blocks; ++b) {
+                    if (!mbar_wait_sleep(&empty_bar[s], ph ^ 1) || *reinterpret_cast<volatile int*>(&s_abort)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* dst = ring + s * kWeightStage;
+                    const int32_t y = static_cast<int32_t>(first) + b * kBlock;
+                    mbar_expect_tx(&full_bar[s], kWeightStage);
+                    load_rows<CHUNKED>(&tmap_dy, dst, a0, y, &full_bar[s]);
+                    load_rows<CHUNKED>(&tmap_x, dst + 2 * kChunkBytes, b0, y, &full_bar[s]);
+                    next_stage();
+                }
+            }
+        }
+    } else if (warp == 1) {    // all lanes walk the loop, an elected one issues (see mbar_wait_warp)
+        const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+        constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+        const uint32_t idesc = umma_idesc(fmt, fmt, 1, 1, kTile, kTile);
+        const uint64_t desc = umma_desc_sw128(0, 1024, kChunkBytes);
+        const uint32_t ring_lo = (smem_u32(ring) & 0x3FFFFu) >> 4;
+        for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            decode(u);
+            if (blocks == 0) continue;
+            if (!mbar_wait_warp(&acc_empty[buf], aph ^ 1)) { ok = false; break; }
+            tc_fence_after_sync();
+            for (int b = 0; b < blocks; ++b) {
+                if (!mbar_wait_warp(&full_bar[s], ph)) { ok = false; break; }
+                const int64_t valid = rows - static_cast<int64_t>(b) * kBlock;
+                int depth = kBlock;
+                if (valid < kBlock) {
+                    depth = tail_depth(static_cast<int>(valid));
+                    clear_tail(ring + s * kWeightStage, static_cast<int>(valid), lane);
+                }
+                tc_fence_after_sync();
+                const uint64_t da = desc + ring_lo + s * (kWeightStage >> 4), db = da + (2 * kChunkBytes >> 4);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < kBlock / 16; ++k)
+                        if (k * 16 < depth) mma_f16_ss(tmem + buf * kTile, da + 128 * k, db + 128 * k, idesc, (b | k) != 0 ? 1u : 0u);
+                    tc_commit(&empty_bar[s]);
+                }
+                __syncwarp();
+                next_stage();
+            }
+            if (!ok) break;
+            if (elect_one()) tc_commit(&acc_full[buf]);
+            __syncwarp();
+            aph ^= buf;
+            buf ^= 1;
+        }
+    } else if (warp >= 6) {
+        RowSum<T> sum(warp - 6, lane);
+        for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            decode(u);
+            sum.clear();
+            for (int b = 0; b < blocks; ++b) {
+                if (!mbar_wait_warp(&full_bar[s], ph)) { ok = false; break; }
+                if (b0 == 0) sum.add(ring + s * kWeightStage, rows - static_cast<int64_t>(b) * kBlock);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty_bar[s]);
+                next_stage();
+            }
+            if (b0 != 0) continue;
+            sum.join();
+            const int c = a0 + (warp - 6) * 32 + (lane & 3) * 8;
+            if (lane < 4 && c < g.n) sum.store(g.db + static_cast<int64_t>(e) * g.n + c);
+        }
+    } else {
+        const int quarter = warp & 3;
+        const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+        uint4* box = turn[quarter];
+        for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+            decode(u);
+            if (ok && blocks > 0) {
+                int passed = 1;
+                if (lane == 0) passed = mbar_wait_sleep(&acc_full[buf], aph) ? 1 : 0;
+                if (__shfl_sync(0xffffffffu, passed, 0) == 0) ok = false;
+            }
+            tc_fence_after_sync();
+            T* out = static_cast<T*>(g.out) + static_cast<int64_t>(e) * g.n * g.cols;
+            for (int c = 0; c < kTile; c += 32) {
+                uint32_t acc[32];
+                if (blocks > 0) {
+                    tmem_ld_2x16(tmem_base + buf * kTile + lane_addr + c, acc);
+                    tc_wait_ld(acc);
+                    if (c + 32 == kTile) {
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+                    }
+                } else {      // no rows: zeros, without the tensor cores
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[i] = 0u;
+                }
+                if (b0 + c >= g.cols) continue;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(acc[8 * q + i]);
+                    box[lane * 4 + (q ^ ((lane >> 1) & 3))] = Vec16<T>::pack(v);      // a phase's lanes in different banks
+                }
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int r = q * 8 + (lane >> 2), p = lane & 3;
+                    const int row = a0 + quarter * 32 + r, col = b0 + c + p * 8;
+                    if (row < g.n && col < g.cols) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * g.cols + col) = box[r * 4 + (p ^ ((r >> 1) & 3))];
+                }
+                __syncwarp();
+            }
+            if (blocks > 0) {
+                aph ^= buf;
+                buf ^= 1;
+            }
+        }
+    }
+    if (!ok) {
+        s_abort = 1;
+        if (g.status != nullptr) atomicExch(g.status, 1);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, 2 * kTile);
+    }
+}
+
+template <typename T, bool CHUNKED>
+int launch_weights(const void* x, const void* dy, const RaggedArgs& g, cudaStream_t st) {
+    CUtensorMap tdy, tx;
+    const uint64_t rows = static_cast<uint64_t>(g.T);
+    if (!(CHUNKED ? make_chunk_map(&tdy, dy, g.n, rows, 0) && make_chunk_map(&tx, x, g.cols, rows, 0)
+                  : make_map(&tdy, dy, g.n, rows, 0, 64) && make_map(&tx, x, g.cols, rows, 0, 64)))
+        return TB200_ERR_DRIVER;
+    static bool attr_set[64] = {};
+    const DeviceInfo& dev = device_info();
+    if (!attr_set[dev.index]) {
+        cudaFuncSetAttribute(ragged_few_weights_kernel<T, CHUNKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(kRingBytes + 1024 + (kMaxExperts + 1) * 4));
+        attr_set[dev.index] = true;
+    }
+    const int64_t units = static_cast<int64_t>(g.experts) * ((g.n + kTile - 1) / kTile) * ((g.cols + kTile - 1) / kTile);
+    const int64_t here = 2 * static_cast<int64_t>(dev.sm_count);
+    launch_chained(ragged_few_weights_kernel<T, CHUNKED>, static_cast<unsigned>(units < here ? units : here),
+                   kThreads + (g.db != nullptr ? kSumWarps * 32 : 0), kRingBytes + 1024 + (static_cast<size_t>(g.experts) + 1) * 4, st, tdy, tx, g);
+    count_launch();
+    return launch_status();
+}
+
 template <typename T, int ROWS, bool GRADS, int SPLIT>
 int launch(const CUtensorMap& tx, const CUtensorMap& tw, const RaggedArgs& g, int64_t ctas, cudaStream_t st) {
     static bool attr_set[64] = {};
@@ -340,6 +565,13 @@ int serve(const void* rows, const void* w, const RaggedArgs& g, int32_t N, int32
 int ragged_few(const void* rows, const void* w, const RaggedArgs& g, int32_t N, int32_t K, bool grads, bool bf16, cudaStream_t st) {
     if (grads) return bf16 ? serve<__nv_bfloat16, true>(rows, w, g, N, K, st) : serve<__half, true>(rows, w, g, N, K, st);
     return bf16 ? serve<__nv_bfloat16, false>(rows, w, g, N, K, st) : serve<__half, false>(rows, w, g, N, K, st);
+}
+
+// g.n and g.cols: of a weight gradient
+int ragged_few_weights(const void* x, const void* dy, const RaggedArgs& g, bool bf16, cudaStream_t st) {
+    const bool chunked = g.n % 64 == 0 && g.cols % 64 == 0;
+    if (bf16) return chunked ? launch_weights<__nv_bfloat16, true>(x, dy, g, st) : launch_weights<__nv_bfloat16, false>(x, dy, g, st);
+    return chunked ? launch_weights<__half, true>(x, dy, g, st) : launch_weights<__half, false>(x, dy, g, st);
 }
 
 }  // namespace tb200
