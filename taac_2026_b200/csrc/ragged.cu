@@ -836,11 +836,20 @@ int checked(int32_t experts, int64_t T, int32_t N, int32_t K, int dtype) {
 }
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
-// Rows an expert up to which the kernel of few rows is taken.  Measured, few rows / pairs, in us: 16 experts, 512 -> 2048, of 32 rows 9.1 /
-// 13.7, of 64 12.3 / 14.0, of 128 15.2 / 14.3, their row gradients 12.2 / 17.4, 18.1 / 17.6, 24.5 / 18.4; 64 experts of 64 rows 30.8 / 40.5
-// and 35.2 / 35.1, of 192 rows 53 / 49 and 56 / 49.  It is taken as well where its 64-row units are no more than the pairs, which
-// start more slowly: 2 experts of 200 rows, 256 -> 256, 5.2 / 7.6; one of 256 rows, 512 -> 512, 7.2 / 8.8.
-constexpr int kFewRows = 64;
+// Whether rows and row gradients go to the kernel of few rows: where the experts have up to 64 rows (128 with a depth of up to 512), and
+// where it is expected to end first.  With the time that an SM takes it for 64 rows x 128 columns x 64 of the depth as the unit, it takes
+// units * blocks / SMs; a round of the pairs' tiles takes 1.09 a block and their start 8.1 more (fitted to the figures
+// below and others between them).  Measured, it / the pairs, in us: 16 experts, 512 -> 2048, of 32 rows 7.5 / 13.2, of 64 11.1 / 13.5, of 128 14.8 / 14.2, of
+// 256 21.9 / 17.8, their row gradients (2048 deep) 11.4 / 15.7, 13.4 / 16.0, 16.0 / 16.8, 26.9 / 17.5; 64 experts of 64 rows 30.4 / 41.5
+// and 34.0 / 33.1; 256 of 128 rows, 512 -> 512, 43.5 / 52.1; one of 4000, 512 -> 512, 7.6 / 9.2; 9 of 512 rows 7.9 / 9.8; 3 of 1500 rows,
+// 1024 -> 512, 14.9 / 12.4; one of 256 rows, 2048 -> 2048, 10.9 / 16.2.
+bool few_rows(const RaggedArgs& g) {
+    const int64_t blocks = (g.depth + kBlock - 1) / kBlock, half = (g.experts + 1) / 2;
+    if (g.T <= 64ll * g.experts || (g.T <= 128ll * g.experts && blocks <= 8)) return true;
+    const int64_t units = (g.T / 64 + half) * ((g.cols + 127) / 128);
+    const int64_t rounds = ((g.T / kTile + half) * ((g.cols + kTile - 1) / kTile) + pairs_here() - 1) / pairs_here();
+    return 100 * units * blocks < 2 * pairs_here() * (109 * rounds * blocks + 810);   // two SMs a pair
+}
 
 template <typename T>
 int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bool grads, cudaStream_t st) {
@@ -849,8 +858,7 @@ int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bo
     const int32_t in = grads ? N : K, out = grads ? K : N;
     g.cols = out;
     g.depth = in;
-    const int64_t few_units = (g.T / 64 + (g.experts + 1) / 2) * ((out + 127) / 128);
-    if (g.T <= kFewRows * static_cast<int64_t>(g.experts) || few_units <= pairs_here()) return ragged_few(x, w, g, N, K, grads, std::is_same<T, __nv_bfloat16>::value, st);
+    if (few_rows(g)) return ragged_few(x, w, g, N, K, grads, std::is_same<T, __nv_bfloat16>::value, st);
     const bool chunked = grads && K % 64 == 0;
     if (!make_map(&ta, x, in, rows, 0, 128) ||
         !(chunked ? make_chunk_map(&tb, w, K, N, g.experts) : make_map(&tb, w, K, N, g.experts, grads ? 64 : 128)) || !make_map(&to, g.out, out, rows, 0, 32))
