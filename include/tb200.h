@@ -527,7 +527,8 @@ int tb200_head_fwd(const void* h, const float* w, const float* bias, float* logi
  *     out[r] = act(x[r] @ w[e]^T + bias[e]) (+ residual[r]),   act: 0 = none, 1 = SiLU
  * offsets: DEVICE int32 [experts + 1], read on the device; an offset outside [0, T] counts as the nearer end, one before an
  * earlier offset as that one.  x, w, residual, out: fp16 or bf16 (dtype), contiguous; bias fp32 [experts, N]; bias and residual may be
- * NULL; residual may be out itself.  Rows that belong to no expert are left as they are (clear = 0) or set to zero.
+ * NULL; residual may be out itself.  Rows that belong to no expert are left as they are (clear = 0) or
+ * hold the residual's values, zeros without one.
  * N % 8 == 0, K % 8 == 0, experts <= 2048.  fp32 accumulation, one rounding.  status_word: as in tb200_gemm_bf16_grouped. */
 int tb200_ragged_gemm(const void* x, const void* w, const int32_t* offsets, const float* bias, const void* residual, void* out,
                       int32_t experts, int64_t T, int32_t N, int32_t K, int32_t act, int32_t clear, int dtype,

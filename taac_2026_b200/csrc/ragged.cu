@@ -527,17 +527,8 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         uint8_t* box = out_s + ew * kBoxBytes;
         const int swz = lane & 7;
         T* out = static_cast<T*>(g.out);
-        if (MODE != kWeights && g.clear) {        // rows in front of the first expert and behind the last
-            const int64_t head = line.begin[0], owned = line.begin[g.experts] - head;
-            const int64_t row_pieces = g.cols / 8, pieces = (g.T - owned) * row_pieces;
-            for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kEpiWarps * 32) + threadIdx.x - 64; i < pieces;
-                 i += static_cast<int64_t>(gridDim.x) * (kEpiWarps * 32)) {
-                int64_t r = i / row_pieces;
-                const int64_t c = i - r * row_pieces;
-                if (r >= head) r += owned;
-                reinterpret_cast<uint4*>(out)[r * row_pieces + c] = make_uint4(0u, 0u, 0u, 0u);
-            }
-        }
+        if (MODE != kWeights && g.clear)
+            rows_of_none(g, line.begin, static_cast<int64_t>(blockIdx.x) * (kEpiWarps * 32) + threadIdx.x - 64, static_cast<int64_t>(gridDim.x) * (kEpiWarps * 32));
         uint32_t buf = 0, aph = 0;
         bool ok = true;
         int4 left0 = make_int4(-1, 0, 0, 0), left1 = left0;
@@ -933,7 +924,11 @@ extern "C" int tb200_ragged_gemm(const void* x, const void* w, const int32_t* of
     if (!aligned16(x) || !aligned16(w) || !aligned16(out) || !aligned16(residual) || !aligned16(bias) || !aligned4(offsets)) return TB200_ERR_ALIGN;
     if (!device_info().valid) return TB200_ERR_DEVICE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (experts == 0) return clear ? static_cast<int>(cudaMemsetAsync(out, 0, static_cast<size_t>(T) * N * 2, st)) : TB200_OK;
+    if (experts == 0) {
+        const size_t bytes = static_cast<size_t>(T) * N * 2;
+        if (!clear || residual == out) return TB200_OK;
+        return static_cast<int>(residual == nullptr ? cudaMemsetAsync(out, 0, bytes, st) : cudaMemcpyAsync(out, residual, bytes, cudaMemcpyDeviceToDevice, st));
+    }
     RaggedArgs g{};
     g.offsets = offsets;
     g.bias = bias;

@@ -26,7 +26,7 @@ struct RaggedArgs {
     int32_t depth;              // contracted length (rows, row grads)
     int32_t n;                  // rows of a weight gradient
     int32_t silu;
-    int32_t clear;              // rows of no expert are set to zero
+    int32_t clear;              // rows of no expert are written too
 };
 
 // Where every expert's rows begin, by one warp; the offsets come from the kernel in front.  An offset outside [0, T] is moved to
@@ -81,6 +81,15 @@ __device__ __forceinline__ int expert_of(const int32_t* pre, int experts, int64_
         else hi = mid;
     }
     return lo;
+}
+// The rows in front of the first expert and behind the last hold the residual's, zeros without one: thread i of n
+__device__ __forceinline__ void rows_of_none(const RaggedArgs& g, const int32_t* begin, int64_t i, int64_t n) {
+    const int64_t head = begin[0], owned = begin[g.experts] - head;
+    const int64_t row_pieces = g.cols / 8, pieces = (g.T - owned) * row_pieces;
+    for (; i < pieces; i += n) {
+        const int64_t at = i < head * row_pieces ? i : i + owned * row_pieces;
+        static_cast<uint4*>(g.out)[at] = g.residual == nullptr ? make_uint4(0u, 0u, 0u, 0u) : static_cast<const uint4*>(g.residual)[at];
+    }
 }
 // ---- weight gradients: stages of 64 contraction rows, as chunks of 64 rows x 128 bytes (MN-major operands, 128-byte swizzle)
 constexpr uint32_t kChunkBytes = 64 * 128;

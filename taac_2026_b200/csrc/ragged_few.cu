@@ -155,16 +155,7 @@ ragged_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
         const int quarter = warp & 3;
         const int mine = quarter * 32 + lane;                   // output column inside the unit = TMEM lane
         const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-        if (g.clear) {                                          // rows in front of the first expert and behind the last
-            const int64_t head = begin[0], owned = begin[g.experts] - head;
-            const int64_t row_pieces = g.cols / 8, pieces = (g.T - owned) * row_pieces;
-            for (int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x - 64; i < pieces; i += static_cast<int64_t>(gridDim.x) * 128) {
-                int64_t r = i / row_pieces;
-                const int64_t c = i - r * row_pieces;
-                if (r >= head) r += owned;
-                static_cast<uint4*>(g.out)[r * row_pieces + c] = make_uint4(0u, 0u, 0u, 0u);
-            }
-        }
+        if (g.clear) rows_of_none(g, begin, static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x - 64, static_cast<int64_t>(gridDim.x) * 128);
         float* part = reinterpret_cast<float*>(ring);
         uint32_t buf = 0, aph = 0;
         for (int64_t u = first_unit; u < units; u += unit_step) {

@@ -1789,8 +1789,8 @@ def ragged_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, 
 
     x: [T, K] with the rows sorted by expert; weight: [E, N, K]; offsets: int32 [E + 1] on the device, not decreasing (one
     that does counts as the largest before it, and all are held inside [0, T]); bias: [E, N] (any float dtype; used as fp32);
-    residual / out: [T, N]; ``out`` may be ``residual``.  fp16 or bf16; N and K are multiples of 8.  Rows of no expert are
-    zero in a fresh result and left as they are in ``out``.
+    residual / out: [T, N]; ``out`` may be ``residual``.  fp16 or bf16; N and K are multiples of 8.  Rows of no expert
+    hold residual's values (zeros without one) in a fresh result and are left as they are in ``out``.
 
     Differentiable in x, weight, bias and residual (without ``silu`` and ``out``).  ``checkpoint=True`` keeps x for the
     weight gradient in 8 bits (``checkpoint_activation``; K a multiple of 128) instead of as it is.  ``check`` / ``status``: as

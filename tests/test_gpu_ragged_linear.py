@@ -139,6 +139,24 @@ def test_rows_of_no_expert(dtype, sizes):
     assert bool((dx[:lead] == 0).all()) and bool((dx[ends[-1]:] == 0).all())
 
 
+@pytest.mark.parametrize("sizes,n,k", [([3, 0, 70, 1], 136, 200), ([1500, 1500], 1024, 1024)])
+def test_residual_of_rows_of_no_expert(sizes, n, k):
+    """In a fresh result those rows are the residual's: what its gradient, the upstream one of every row, says too."""
+    lead, behind = 37, 90
+    x, w, off, dy, bias, ends = _case(sizes, n, k, torch.bfloat16, 15, lead, behind)
+    res = torch.randn_like(dy).requires_grad_()
+    out = ops.ragged_linear(x, w, off, bias, residual=res)
+    _check_rows(out.detach(), x, w, ends, bias, False, res.detach())
+    assert torch.equal(out[:lead], res[:lead]) and torch.equal(out[ends[-1]:], res[ends[-1]:])
+    out.backward(dy)
+    assert torch.equal(res.grad, dy)
+    into = res.detach().clone()
+    assert torch.equal(ops.ragged_linear(x, w, off, bias, residual=into, out=into), out)
+    none = ops.ragged_linear(x, w[:0], off[:1], residual=res.detach())
+    assert torch.equal(none, res)
+    assert bool((ops.ragged_linear(x, w[:0], off[:1]) == 0).all())
+
+
 def test_one_experts_nan_stays_with_it():
     sizes = [100, 30, 200, 64]
     x, w, off, dy, bias, ends = _case(sizes, 256, 128, torch.bfloat16, 8)
@@ -330,6 +348,23 @@ def test_tiles_shared_by_pairs(sizes):
     _check_grads(dx, dw, db, x, w, dy, ends)
     again = ops.ragged_linear_backward(x, w, off, dy, bias=True)
     assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), again))
+
+
+EDGES = [1, 0, 31, 32, 33, 127, 128, 129, 255, 256, 257, 1500, 900]
+
+
+@pytest.mark.parametrize("sizes,n,k", [(EDGES, 1000, 520), (EDGES, 1000, 512), ([5000, 0, 1, 3000, 4097, 70], 1000, 520), ([5000, 0, 1, 3000, 4097, 70], 1024, 512),
+                                       ([17000, 60, 1], 520, 264), ([0, 1, 20000, 0], 264, 512), ([150, 151, 163] * 500, 512, 64), ([800, 790, 830] * 100, 136, 72)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tiles_of_pairs(sizes, n, k, dtype):
+    """Sizes at the edges of a tile, a quarter and a warp, experts without rows and many experts, in sums large enough for CTA pairs
+    (the first two and the 1500 experts: rows and their gradients; the others: weight gradients)."""
+    x, w, off, dy, bias, ends = _case(sizes, n, k, dtype, 41, 5, 3)
+    _check_rows(ops.ragged_linear(x, w, off, bias, residual=dy, check=True), x, w, ends, bias, False, dy)
+    _check_rows(ops.ragged_linear(x, w, off, bias, silu=True, check=True), x, w, ends, bias, True)
+    dx, dw, db = ops.ragged_linear_backward(x, w, off, dy, bias=True, check=True)
+    _check_grads(dx, dw, db, x, w, dy, ends)
+    assert bool((dx[:5] == 0).all()) and bool((dx[-3:] == 0).all())
 
 
 @pytest.mark.parametrize("sizes,n,k", [([3, 1, 0, 2], 512, 1024), ([30, 20], 256, 2048), ([60, 64, 65], 128, 4096), ([1], 2048, 1024), ([17] * 70, 136, 520)])
