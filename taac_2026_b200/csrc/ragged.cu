@@ -592,10 +592,10 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                 } else {
                     __syncwarp();
                 }
-                if (MODE == kWeights && part != nullptr) {
+                if (MODE == kWeights && part != nullptr) {         // what lies outside dw is not read again
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
-                        *reinterpret_cast<uint4*>(part + static_cast<int64_t>(half * 32 + piece * 8 + q) * 512) =
+                        if (live && col + 4 * q < g.cols) *reinterpret_cast<uint4*>(part + static_cast<int64_t>(half * 32 + piece * 8 + q) * 512) =
                             make_uint4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
                     continue;
                 }
@@ -664,50 +664,70 @@ ragged_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
 }
 
 // Adds the partial tiles of every shared weight-gradient tile.  CTA (x, y): if pair x left the begin of a tile, what the pairs behind it
-// left of the same tile is added to it, in their order, for 32 of the tile's columns (a thread holds one of the 256 rows).
+// left of the same tile is added to it, in their order, for kJoinCols of the tile's columns (a thread holds one of the 256 rows).  One
+// tile may be shared by all pairs, so four partial tiles are loaded at a time.  One expert of 60000 rows, 512 -> 512 (18 pairs a tile),
+// with the products: 66.9 us with one at a time and 32 columns a CTA, 53.5 so, 56.5 with 8 columns, 55.7 with CTAs that walk a list of
+// the shared tiles (which costs 172.7 for 156.1 where many are shared).
+constexpr int kJoinCols = 16;
 template <typename T>
 __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, int pairs) {
+    constexpr int kQuads = kJoinCols / 4, kAhead = 4;
     chain_release();
     chain_wait();
     const int4 mine = __ldcg(g.pieces + 2 * blockIdx.x + 1);
-    if (mine.x < 0) return;
-    const int r = threadIdx.x;
-    if (blockIdx.y == 0 && g.db != nullptr && mine.z == 0 && mine.y + r < g.n) {
-        float sum = __ldcg(g.db_partial + (2 * static_cast<int64_t>(blockIdx.x) + 1) * kTile + r);
-        for (int k = blockIdx.x + 1; k < pairs; ++k) {
-            const int4 next = __ldcg(g.pieces + 2 * k);
-            if (next.x < 0) continue;
-            sum += __ldcg(g.db_partial + 2 * static_cast<int64_t>(k) * kTile + r);
-            if (next.w != 0) break;
-        }
-        g.db[static_cast<int64_t>(mine.x) * g.n + mine.y + r] = sum;
-    }
-    const int row = mine.y + r, col = mine.z + blockIdx.y * 32;
-    float4 sum[8];
-    auto add = [&](int pair, int slot, bool first) {
-        const float* part = g.partial + (static_cast<int64_t>(pair) * 2 + slot) * kPartFloats + (r >> 7) * (kPartFloats / 2) + (r & 127) * 4;
+    const int r = threadIdx.x, lane = threadIdx.x & 31;
+    const int row = mine.y + r, col = mine.z + blockIdx.y * kJoinCols;
+    if (mine.x < 0 || col >= g.cols) return;
+    const bool live = row < g.n, biased = blockIdx.y == 0 && g.db != nullptr && mine.z == 0 && live;
+    const float* part = g.partial + (r >> 7) * (kPartFloats / 2) + static_cast<int64_t>(blockIdx.y) * (kQuads * 512) + (r & 127) * 4;
+    float4 sum[kQuads];
+    float db = 0.f;
+    if (live) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part + static_cast<int64_t>(blockIdx.y * 8 + q) * 512));
-            if (first) sum[q] = v;
-            else sum[q] = make_float4(sum[q].x + v.x, sum[q].y + v.y, sum[q].z + v.z, sum[q].w + v.w);
-        }
-    };
-    add(blockIdx.x, 1, true);
-    for (int k = blockIdx.x + 1; k < pairs; ++k) {
-        const int4 next = __ldcg(g.pieces + 2 * k);
-        if (next.x < 0) continue;      // a pair without a share
-        add(k, 0, false);
-        if (next.w != 0) break;
+        for (int q = 0; q < kQuads; ++q) sum[q] = __ldcg(reinterpret_cast<const float4*>(part + (2 * static_cast<int64_t>(blockIdx.x) + 1) * kPartFloats + q * 512));
+        if (biased) db = __ldcg(g.db_partial + (2 * static_cast<int64_t>(blockIdx.x) + 1) * kTile + r);
     }
-    if (row >= g.n) return;
+    bool more = true;
+    for (int base = blockIdx.x + 1; more && base < pairs; base += 32) {
+        // the pairs with a share of the tile, up to the one that has its end
+        const int4 piece = base + lane < pairs ? __ldcg(g.pieces + 2 * (base + lane)) : make_int4(-1, 0, 0, 0);
+        uint32_t with = __ballot_sync(0xffffffffu, piece.x >= 0);
+        const uint32_t end = __ballot_sync(0xffffffffu, piece.x >= 0 && piece.w != 0);
+        if (end != 0) {
+            with &= end ^ (end - 1);
+            more = false;
+        }
+        while (with != 0) {
+            float4 v[kAhead][kQuads];
+            float b[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const bool there = with != 0 && live;
+                const int64_t slot = 2 * static_cast<int64_t>(base + (with != 0 ? __ffs(with) - 1 : 0));
+                with &= with - 1;
+                b[k] = there && biased ? __ldcg(g.db_partial + slot * kTile + r) : 0.f;
+#pragma unroll
+                for (int q = 0; q < kQuads; ++q)
+                    v[k][q] = there ? __ldcg(reinterpret_cast<const float4*>(part + slot * kPartFloats + q * 512)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                db += b[k];
+#pragma unroll
+                for (int q = 0; q < kQuads; ++q)
+                    sum[q] = make_float4(sum[q].x + v[k][q].x, sum[q].y + v[k][q].y, sum[q].z + v[k][q].z, sum[q].w + v[k][q].w);
+            }
+        }
+    }
+    if (!live) return;
+    if (biased) g.db[static_cast<int64_t>(mine.x) * g.n + row] = db;
     T* out = static_cast<T*>(g.out) + (static_cast<int64_t>(mine.x) * g.n + row) * g.cols;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        if (col + q * 8 >= g.cols) break;
-        const float4 a = sum[2 * q], b = sum[2 * q + 1];
+    for (int q = 0; q < kQuads; q += 2) {
+        if (col + q * 4 >= g.cols) break;
+        const float4 a = sum[q], b = sum[q + 1];
         const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        *reinterpret_cast<uint4*>(out + col + q * 8) = Vec16<T>::pack(v);
+        *reinterpret_cast<uint4*>(out + col + q * 4) = Vec16<T>::pack(v);
     }
 }
 
@@ -864,17 +884,27 @@ int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bo
 // rows from which on a tile can be shared by pairs: with fewer, no expert has 2 kSnap blocks
 constexpr int64_t kShareRows = 2 * kSnap * kBlock;
 
-// Weight gradients go to the kernel of 128 x 128 tiles while the experts have up to kFewDepth rows each, or up to kFewLong where the 256 x
-// 256 tiles are no more than half of the pairs.  Measured, it / the pairs, with a bias gradient, in us: 16 experts of 128 rows, 512 ->
-// 2048, 15.8 / 20.4, of 512 29.1 / 30.0, of 1024 49.6 / 46.5; 256 of 128 rows, 512 -> 512, 48 / 61; 9 of 2048 rows, 512 -> 512 (36
-// tiles), 26 / 29; one of 1000, 512 -> 512 (4), 13 / 30; 3 of 5000, 1024 -> 512 (24), 65 / 41.
-constexpr int64_t kFewDepth = 768, kFewLong = 4096;
+// Whether the weight gradients go to the kernel of 128 x 128 tiles: where it is expected to end first, by times (in hundredths of a us) that
+// come close to those measured over all sizes.  There a CTA takes 0.65 us a block of 64 rows and five blocks' time a tile at least, two CTAs
+// share an SM, and clusters add 3 us.  Here a pair takes 0.53 us a block and seven blocks' time at least, with whole tiles or in equal
+// shares; the partial tiles of those and their sum, of as many as share a tile, come on top.  Measured, 128 x 128 / pairs, with a
+// bias gradient, in us: 16 experts of 128 rows, 512 -> 2048, 15.8 / 20.4, of 512 29.1 / 30.0, of 1024 49.6 / 46.5; 256 of 128 rows, 512 -> 512,
+// 48 / 61; one of 1000, 512 -> 512, 10.2 / 21.0, of 8000 17.5 / 27.0, of 60000 75.6 / 54.2; 20 of 1500, 256 -> 256, 17.2 / 25.3; 2 of 3000,
+// 512 -> 2048, 24.9 / 33.1; 4 of 10000, 1024 -> 1024, 132.8 / 108.8; one of 100000, 128 -> 128, 102.9 / 58.5.
+bool few_weights(const RaggedArgs& g) {
+    const auto tiles = [&](int tile) { return static_cast<int64_t>(g.experts) * ((g.n + tile - 1) / tile) * ((g.cols + tile - 1) / tile); };
+    const int64_t blocks = (g.T / g.experts + kBlock - 1) / kBlock, small = tiles(128), large = tiles(kTile), pairs = pairs_here(), here = 4 * pairs;
+    const int64_t split = weights_split(small, blocks, here), part = (blocks + split - 1) / split;
+    const int64_t few = (split > 1 ? 900 : 600) + 65 * ((small * split + here - 1) / here) * (part > 5 ? part : 5);
+    const int64_t length = blocks > 7 ? blocks : 7;
+    const int64_t whole = 1200 + 53 * ((large + pairs - 1) / pairs) * length;
+    const int64_t shared = 1500 + 45 * pairs / large + 53 * large * length / pairs;
+    return few < (whole < shared ? whole : shared);
+}
 
 template <typename T>
 int weights_of(const void* x, const void* dy, RaggedArgs g, cudaStream_t st) {
-    const int64_t tiles = static_cast<int64_t>(g.experts) * ((g.n + kTile - 1) / kTile) * ((g.cols + kTile - 1) / kTile);
-    if (g.T <= kFewDepth * g.experts || (2 * tiles <= pairs_here() && g.T <= kFewLong * g.experts))
-        return ragged_few_weights(x, dy, g, std::is_same<T, __nv_bfloat16>::value, st);
+    if (few_weights(g)) return ragged_few_weights(x, dy, g, std::is_same<T, __nv_bfloat16>::value, st);
     CUtensorMap ta, tb, to;
     const uint64_t rows = static_cast<uint64_t>(g.T);
     const bool chunked = g.n % 64 == 0 && g.cols % 64 == 0;
@@ -884,7 +914,7 @@ int weights_of(const void* x, const void* dy, RaggedArgs g, cudaStream_t st) {
     const int pairs = pairs_here();
     const int code = chunked ? launch_pairs<T, kWeights, false, true>(ta, tb, to, g, pairs, st) : launch_pairs<T, kWeights, false, false>(ta, tb, to, g, pairs, st);
     if (code != TB200_OK || g.partial == nullptr) return code;
-    launch_chained(ragged_join_kernel<T>, dim3(pairs, kTile / 32), 256, 0, st, g, pairs);
+    launch_chained(ragged_join_kernel<T>, dim3(pairs, kTile / kJoinCols), 256, 0, st, g, pairs);
     count_launch();
     return launch_status();
 }

@@ -277,10 +277,16 @@ ragged_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
 // Both operands are MN-major, contracted over the expert's rows, the rows of the next expert in a last block cleared by the warp
 // that issues the MMAs; warps 2 to 5 turn the accumulator in shared memory, 32 columns at a time, so that four lanes write 64 bytes
 // of a row; warps 6 to 9 add the rows of dy for the bias gradient.
+//
+// The layers of a model with many rows and narrow weights have few tiles, each a long contraction that a CTA's ring bounds (0.5 to 0.65 us a
+// block, three stages in flight).  SPLIT CTAs of a cluster then take a part of the blocks each and leave partial tiles in their shared memory,
+// of which every rank adds some rows, in the order of the ranks.  One expert of 8000 rows, 512 -> 512, in eight: 17.5 us, 39 without.
+// The sums over the cluster take 2 us in two parts and 3.5 in eight; read by octets, two loads of 16 bytes 32 apart, they took 9.
 constexpr int kSumWarps = 4;
 constexpr uint32_t kWeightStage = 4 * kChunkBytes;
+static_assert(kTile * (kTile + 4) * 4 <= kRingBytes, "a partial tile fits the ring");
 
-template <typename T, bool CHUNKED>
+template <typename T, bool CHUNKED, int SPLIT>
 __global__ void __launch_bounds__(kThreads + kSumWarps * 32, 2)
 ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __grid_constant__ CUtensorMap tmap_x, const RaggedArgs g) {
     extern __shared__ uint8_t smem_raw[];
@@ -288,7 +294,9 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
     __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int s_abort;
-    __shared__ __align__(16) uint4 turn[4][32 * 4];             // a warp's 32 rows x 64 bytes
+    __shared__ __align__(16) uint4 turn[SPLIT > 1 ? 1 : 4][32 * 4];             // a warp's 32 rows x 64 bytes
+    __shared__ __align__(16) float db_part[SPLIT > 1 ? kTile : 4];
+    constexpr int kPartStride = kTile + 4;                      // floats between the rows of a partial tile
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     int32_t* begin = reinterpret_cast<int32_t*>(ring + kStages * kWeightStage);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -324,7 +332,9 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
 
     const int b_tiles = (g.cols + kTile - 1) / kTile, tiles = (g.n + kTile - 1) / kTile * b_tiles;
     const int64_t units = static_cast<int64_t>(g.experts) * tiles;
-    int e, a0, b0, blocks;
+    const int rank = SPLIT > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int64_t first_unit = blockIdx.x / SPLIT, unit_step = gridDim.x / SPLIT;      // with a split a cluster has one unit
+    int e, a0, b0, blocks, block0, block1;                      // blocks of the tile; this CTA's
     int64_t first, rows;
     auto decode = [&](int64_t u) {
         e = static_cast<int>(u / tiles);
@@ -334,6 +344,8 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
         first = begin[e];
         rows = begin[e + 1] - first;
         blocks = static_cast<int>((rows + kBlock - 1) / kBlock);
+        block0 = static_cast<int>(static_cast<int64_t>(blocks) * rank / SPLIT);
+        block1 = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / SPLIT);
     };
     uint32_t s = 0, ph = 0, buf = 0, aph = 0;
     auto next_stage = [&]() {
@@ -345,9 +357,9 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
-            for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            for (int64_t u = first_unit; u < units && ok; u += unit_step) {
                 decode(u);
-                for (int b = 0; b < blocks; ++b) {
+                for (int b = block0; b < block1; ++b) {
                     if (!mbar_wait_sleep(&empty_bar[s], ph ^ 1) || *reinterpret_cast<volatile int*>(&s_abort)) {
                         ok = false;
                         break;
@@ -367,12 +379,12 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
         const uint32_t idesc = umma_idesc(fmt, fmt, 1, 1, kTile, kTile);
         const uint64_t desc = umma_desc_sw128(0, 1024, kChunkBytes);
         const uint32_t ring_lo = (smem_u32(ring) & 0x3FFFFu) >> 4;
-        for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        for (int64_t u = first_unit; u < units && ok; u += unit_step) {
             decode(u);
-            if (blocks == 0) continue;
+            if (block0 == block1) continue;
             if (!mbar_wait_warp(&acc_empty[buf], aph ^ 1)) { ok = false; break; }
             tc_fence_after_sync();
-            for (int b = 0; b < blocks; ++b) {
+            for (int b = block0; b < block1; ++b) {
                 if (!mbar_wait_warp(&full_bar[s], ph)) { ok = false; break; }
                 const int64_t valid = rows - static_cast<int64_t>(b) * kBlock;
                 int depth = kBlock;
@@ -385,7 +397,7 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < kBlock / 16; ++k)
-                        if (k * 16 < depth) mma_f16_ss(tmem + buf * kTile, da + 128 * k, db + 128 * k, idesc, (b | k) != 0 ? 1u : 0u);
+                        if (k * 16 < depth) mma_f16_ss(tmem + buf * kTile, da + 128 * k, db + 128 * k, idesc, b > block0 || k > 0 ? 1u : 0u);
                     tc_commit(&empty_bar[s]);
                 }
                 __syncwarp();
@@ -399,10 +411,10 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
         }
     } else if (warp >= 6) {
         RowSum<T> sum(warp - 6, lane);
-        for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        for (int64_t u = first_unit; u < units && ok; u += unit_step) {
             decode(u);
             sum.clear();
-            for (int b = 0; b < blocks; ++b) {
+            for (int b = block0; b < block1; ++b) {
                 if (!mbar_wait_warp(&full_bar[s], ph)) { ok = false; break; }
                 if (b0 == 0) sum.add(ring + s * kWeightStage, rows - static_cast<int64_t>(b) * kBlock);
                 __syncwarp();
@@ -412,20 +424,38 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
             if (b0 != 0) continue;
             sum.join();
             const int c = a0 + (warp - 6) * 32 + (lane & 3) * 8;
-            if (lane < 4 && c < g.n) sum.store(g.db + static_cast<int64_t>(e) * g.n + c);
+            if (SPLIT > 1 && lane < 4) sum.store(db_part + (warp - 6) * 32 + (lane & 3) * 8);
+            else if (lane < 4 && c < g.n) sum.store(g.db + static_cast<int64_t>(e) * g.n + c);
+        }
+        if (SPLIT > 1) {                                            // done with the ring
+            __syncwarp();
+            asm volatile("bar.arrive 1, 256;" ::: "memory");
         }
     } else {
         const int quarter = warp & 3;
         const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
         uint4* box = turn[quarter];
-        for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        for (int64_t u = first_unit; u < units; u += unit_step) {
             decode(u);
-            if (ok && blocks > 0) {
+            if (ok && block0 < block1) {
                 int passed = 1;
                 if (lane == 0) passed = mbar_wait_sleep(&acc_full[buf], aph) ? 1 : 0;
                 if (__shfl_sync(0xffffffffu, passed, 0) == 0) ok = false;
             }
             tc_fence_after_sync();
+            if (SPLIT > 1) {                                        // the partial tile, into the ring: the MMAs have read it, the bias warps too
+                if (g.db != nullptr) asm volatile("bar.sync 1, 256;" ::: "memory");
+                float* part = reinterpret_cast<float*>(ring) + (quarter * 32 + lane) * kPartStride;
+                for (int c = 0; c < kTile && block0 < block1; c += 32) {
+                    uint32_t acc[32];
+                    tmem_ld_2x16(tmem_base + buf * kTile + lane_addr + c, acc);
+                    tc_wait_ld(acc);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        *reinterpret_cast<uint4*>(part + c + 4 * q) = make_uint4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+                }
+                continue;
+            }
             T* out = static_cast<T*>(g.out) + static_cast<int64_t>(e) * g.n * g.cols;
             for (int c = 0; c < kTile; c += 32) {
                 uint32_t acc[32];
@@ -464,6 +494,49 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
             }
         }
     }
+    if (SPLIT > 1) {
+        __syncwarp();
+        cluster_sync_all();                                     // every rank's partial tile is in place
+        if (warp >= 2) {
+            decode(first_unit);
+            const uint32_t at = smem_u32(ring);
+            const int t = threadIdx.x - 64, threads = blockDim.x - 64;
+            constexpr int kItems = kTile / SPLIT * (kTile / 4), kBatch = SPLIT < 8 ? 8 / SPLIT : 1;      // four columns of one of this rank's rows
+            for (int i0 = t; i0 < kItems; i0 += kBatch * threads) {
+                float4 v[kBatch][SPLIT];
+                int r[kBatch], c[kBatch];
+                bool live[kBatch];
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    const int i = i0 + b * threads;
+                    r[b] = rank * (kTile / SPLIT) + i / (kTile / 4);
+                    c[b] = i % (kTile / 4) * 4;
+                    live[b] = i < kItems && a0 + r[b] < g.n && b0 + c[b] < g.cols;
+#pragma unroll
+                    for (int k = 0; k < SPLIT; ++k) {
+                        const bool there = live[b] && static_cast<int64_t>(blocks) * k / SPLIT < static_cast<int64_t>(blocks) * (k + 1) / SPLIT;
+                        v[b][k] = there ? ld_peer4(at + (r[b] * kPartStride + c[b]) * 4, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    float4 sum = v[b][0];
+#pragma unroll
+                    for (int k = 1; k < SPLIT; ++k) sum = make_float4(sum.x + v[b][k].x, sum.y + v[b][k].y, sum.z + v[b][k].z, sum.w + v[b][k].w);
+                    __align__(8) const T out[4] = {from_float<T>(sum.x), from_float<T>(sum.y), from_float<T>(sum.z), from_float<T>(sum.w)};
+                    if (live[b]) *reinterpret_cast<uint2*>(static_cast<T*>(g.out) + (static_cast<int64_t>(e) * g.n + a0 + r[b]) * g.cols + b0 + c[b]) = *reinterpret_cast<const uint2*>(out);
+                }
+            }
+            if (g.db != nullptr && rank == 0 && b0 == 0 && t < kTile && a0 + t < g.n) {
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < SPLIT; ++k) sum += ld_peer(smem_u32(db_part) + t * 4, k);
+                g.db[static_cast<int64_t>(e) * g.n + a0 + t] = sum;
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();                                     // nobody leaves while its partial tile is being read
+    }
     if (!ok) {
         s_abort = 1;
         if (g.status != nullptr) atomicExch(g.status, 1);
@@ -476,26 +549,55 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
     }
 }
 
+// `ctas` of `threads` in clusters of `split`, which may start while the kernel in front still runs
+template <typename K, typename... Args>
+int launch_clusters(K kernel, int split, int64_t ctas, int threads, size_t smem, cudaStream_t st, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = static_cast<unsigned>(ctas);
+    cfg.blockDim = static_cast<unsigned>(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = split > 1 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, args...);
+    count_launch();
+    return launch_status();
+}
+
+template <typename T, bool CHUNKED, int SPLIT>
+int launch_weights(const CUtensorMap& tdy, const CUtensorMap& tx, const RaggedArgs& g, int64_t ctas, cudaStream_t st) {
+    static bool attr_set[64] = {};
+    const DeviceInfo& dev = device_info();
+    if (!attr_set[dev.index]) {
+        cudaFuncSetAttribute(ragged_few_weights_kernel<T, CHUNKED, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(kRingBytes + 1024 + (kMaxExperts + 1) * 4));
+        attr_set[dev.index] = true;
+    }
+    return launch_clusters(ragged_few_weights_kernel<T, CHUNKED, SPLIT>, SPLIT, ctas, kThreads + (g.db != nullptr ? kSumWarps * 32 : 0),
+                           kRingBytes + 1024 + (static_cast<size_t>(g.experts) + 1) * 4, st, tdy, tx, g);
+}
+
 template <typename T, bool CHUNKED>
-int launch_weights(const void* x, const void* dy, const RaggedArgs& g, cudaStream_t st) {
+int split_weights(const void* x, const void* dy, const RaggedArgs& g, cudaStream_t st) {
     CUtensorMap tdy, tx;
     const uint64_t rows = static_cast<uint64_t>(g.T);
     if (!(CHUNKED ? make_chunk_map(&tdy, dy, g.n, rows, 0) && make_chunk_map(&tx, x, g.cols, rows, 0)
                   : make_map(&tdy, dy, g.n, rows, 0, 64) && make_map(&tx, x, g.cols, rows, 0, 64)))
         return TB200_ERR_DRIVER;
-    static bool attr_set[64] = {};
-    const DeviceInfo& dev = device_info();
-    if (!attr_set[dev.index]) {
-        cudaFuncSetAttribute(ragged_few_weights_kernel<T, CHUNKED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(kRingBytes + 1024 + (kMaxExperts + 1) * 4));
-        attr_set[dev.index] = true;
-    }
     const int64_t units = static_cast<int64_t>(g.experts) * ((g.n + kTile - 1) / kTile) * ((g.cols + kTile - 1) / kTile);
-    const int64_t here = 2 * static_cast<int64_t>(dev.sm_count);
-    launch_chained(ragged_few_weights_kernel<T, CHUNKED>, static_cast<unsigned>(units < here ? units : here),
-                   kThreads + (g.db != nullptr ? kSumWarps * 32 : 0), kRingBytes + 1024 + (static_cast<size_t>(g.experts) + 1) * 4, st, tdy, tx, g);
-    count_launch();
-    return launch_status();
+    const int64_t here = 2 * static_cast<int64_t>(device_info().sm_count);
+    switch (weights_split(units, (g.T / g.experts + kBlock - 1) / kBlock, here)) {
+        case 8: return launch_weights<T, CHUNKED, 8>(tdy, tx, g, 8 * units, st);
+        case 4: return launch_weights<T, CHUNKED, 4>(tdy, tx, g, 4 * units, st);
+        case 2: return launch_weights<T, CHUNKED, 2>(tdy, tx, g, 2 * units, st);
+        default: return launch_weights<T, CHUNKED, 1>(tdy, tx, g, units < here ? units : here, st);
+    }
 }
 
 template <typename T, int ROWS, bool GRADS, int SPLIT>
@@ -507,22 +609,7 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, const RaggedArgs& g, in
                              static_cast<int>(kRingBytes + 1024 + (kMaxExperts + 1) * 8));
         attr_set[dev.index] = true;
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = static_cast<unsigned>(ctas);
-    cfg.blockDim = kThreads;
-    cfg.dynamicSmemBytes = kRingBytes + 1024 + (static_cast<size_t>(g.experts) + 1) * 8;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2]{};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = SPLIT;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = SPLIT > 1 ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, ragged_few_kernel<T, ROWS, GRADS, SPLIT>, tx, tw, g);
-    count_launch();
-    return launch_status();
+    return launch_clusters(ragged_few_kernel<T, ROWS, GRADS, SPLIT>, SPLIT, ctas, kThreads, kRingBytes + 1024 + (static_cast<size_t>(g.experts) + 1) * 8, st, tx, tw, g);
 }
 
 template <typename T, int ROWS, bool GRADS>
@@ -561,8 +648,8 @@ int ragged_few(const void* rows, const void* w, const RaggedArgs& g, int32_t N, 
 // g.n and g.cols: of a weight gradient
 int ragged_few_weights(const void* x, const void* dy, const RaggedArgs& g, bool bf16, cudaStream_t st) {
     const bool chunked = g.n % 64 == 0 && g.cols % 64 == 0;
-    if (bf16) return chunked ? launch_weights<__nv_bfloat16, true>(x, dy, g, st) : launch_weights<__nv_bfloat16, false>(x, dy, g, st);
-    return chunked ? launch_weights<__half, true>(x, dy, g, st) : launch_weights<__half, false>(x, dy, g, st);
+    if (bf16) return chunked ? split_weights<__nv_bfloat16, true>(x, dy, g, st) : split_weights<__nv_bfloat16, false>(x, dy, g, st);
+    return chunked ? split_weights<__half, true>(x, dy, g, st) : split_weights<__half, false>(x, dy, g, st);
 }
 
 }  // namespace tb200

@@ -145,6 +145,13 @@ __device__ __forceinline__ float ld_peer(uint32_t smem_addr, uint32_t rank) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
     return v;
 }
+__device__ __forceinline__ float4 ld_peer4(uint32_t smem_addr, uint32_t rank) {
+    uint32_t at;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+    return v;
+}
 
 // ---------------------------------------------------------------------------
 // proxy fences

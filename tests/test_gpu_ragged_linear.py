@@ -72,9 +72,17 @@ def _check_grads(dx, dw, db, x, w, dy, ends):
     dtype, n = dx.dtype, w.shape[1]
     for e in range(len(ends) - 1):
         r = slice(ends[e], ends[e + 1])
-        xe, we, ge = x[r].double(), w[e].double(), dy[r].double()
+        we, ge = w[e].double(), dy[r].double()
         want = ge @ we
         _within(dx[r], want, _half(dtype) * want.abs() + _steps(n) * (ge.abs() @ we.abs()) + _tiny(dtype))
+    _check_weights(dw, db, x, dy, ends)
+
+
+def _check_weights(dw, db, x, dy, ends):
+    dtype = dw.dtype
+    for e in range(len(ends) - 1):
+        r = slice(ends[e], ends[e + 1])
+        xe, ge = x[r].double(), dy[r].double()
         want = ge.T @ xe
         _within(dw[e], want, _half(dtype) * want.abs() + _steps(len(xe)) * (ge.abs().T @ xe.abs()) + _tiny(dtype))
         if db is not None:      # fp32: every eighth row in order in a lane (in a thread of 1 to 8 without dw), then 3 + 74 or 8 + 74 partial sums
@@ -348,6 +356,19 @@ def test_tiles_shared_by_pairs(sizes):
     _check_grads(dx, dw, db, x, w, dy, ends)
     again = ops.ragged_linear_backward(x, w, off, dy, bias=True)
     assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), again))
+
+
+@pytest.mark.parametrize("sizes,n,k", [([1000, 900], 512, 512), ([2200, 0, 5, 4000], 136, 72), ([3000], 128, 256), ([0, 9000, 1], 264, 200), ([130, 3500, 64], 512, 128)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weight_gradients_in_parts(sizes, n, k, dtype):
+    """Few tiles with long contractions, a part of them for each CTA of a cluster of two, four or eight; some ranks have no rows."""
+    x, w, off, dy, bias, ends = _case(sizes, n, k, dtype, 51, 3, 70)
+    x[:3], x[-70:], dy[:3], dy[-70:] = float("nan"), float("inf"), float("nan"), float("nan")
+    for biased in (True, False):
+        _dx, dw, db = ops.ragged_linear_backward(x, w, off, dy, bias=biased, need_x=False, check=True)
+        _check_weights(dw, db, x, dy, ends)
+        again = ops.ragged_linear_backward(x, w, off, dy, bias=biased, need_x=False)
+        assert torch.equal(dw, again[1]) and (not biased or torch.equal(db, again[2]))
 
 
 EDGES = [1, 0, 31, 32, 33, 127, 128, 129, 255, 256, 257, 1500, 900]
