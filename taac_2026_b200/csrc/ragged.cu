@@ -20,8 +20,11 @@
 //
 // Distribution.  Row tiles go round robin over the pairs.  The tiles of the weight gradients of uneven experts differ in
 // length: they go round robin as well, the long ones first, unless that would leave pairs idle for long; then the rest is cut into
-// shares that even the pairs out (see Line), and a tile that two or more pairs share leaves fp32 partial tiles in a workspace, which `ragged_join_kernel` adds in the order of the pairs.  The bias
-// gradient comes with the weight gradient: four more warps add the rows of dy that lie in shared memory.
+// shares that even the pairs out (see Line), and a tile that two or more pairs share leaves fp32 partial tiles in a workspace, which
+// `ragged_join_kernel` adds in the order of the pairs.  The bias gradient comes with the weight gradient: four more warps add the
+// rows of dy that lie in shared memory.
+//
+// Layers with few rows an expert or few tiles go to the kernels of ragged_few.cu (see few_rows and few_weights).
 //
 // Every wait on an mbarrier is bounded; a wait that gives up raises the status word and all roles drain through the final barrier.
 #include "ragged.cuh"
@@ -731,8 +734,8 @@ __global__ void __launch_bounds__(256) ragged_join_kernel(const RaggedArgs g, in
     }
 }
 
-// db[e] = sum of the expert's rows of dy where no weight gradient is wanted, in two steps of fixed order.  Step one: CTA (x, y) adds the rows of chunk x, `chunk` rows
-// of the matrix, for blockDim.x * 8 columns, and leaves a partial sum for every expert that has rows among them; that of
+// db[e] = sum of the expert's rows of dy where no weight gradient is wanted, in two steps of fixed order.  Step one: CTA (x, y) adds the
+// rows of chunk x, `chunk` rows of the matrix, for blockDim.x * 8 columns, and leaves a partial sum for every expert that has rows among them; that of
 // expert e stands in row x + e of the table, which no other pair of chunk and expert has, for both grow along the matrix.
 // Thread (tx, ty) takes eight columns of every blockDim.y-th row, eight loads in flight.  As many chunks as CTAs fit the chip:
 // pieces of 32 rows of one expert, a CTA each, took 42 us instead of 24 for 32768 x 2048, start-up and waves of CTAs.
@@ -876,7 +879,8 @@ int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bo
         return TB200_ERR_DRIVER;
     const int64_t most = (g.T / kTile + g.experts) * ((out + kTile - 1) / kTile);
     const int pairs = static_cast<int>(most < pairs_here() ? most : pairs_here());
-    if (grads) return chunked ? launch_pairs<T, kRowGrads, false, true>(ta, tb, to, g, pairs, st) : launch_pairs<T, kRowGrads, false, false>(ta, tb, to, g, pairs, st);
+    if (chunked) return launch_pairs<T, kRowGrads, false, true>(ta, tb, to, g, pairs, st);
+    if (grads) return launch_pairs<T, kRowGrads, false, false>(ta, tb, to, g, pairs, st);
     if (g.residual != nullptr) return launch_pairs<T, kRows, true, false>(ta, tb, to, g, pairs, st);
     return launch_pairs<T, kRows, false, false>(ta, tb, to, g, pairs, st);
 }

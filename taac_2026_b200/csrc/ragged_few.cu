@@ -13,7 +13,8 @@
 // Where the units are fewer than the SMs can take and the contraction is long, SPLIT CTAs of a cluster take a part of it each
 // and the partial sums, left in shared memory, are added in the order of the ranks, every rank some of the rows.
 //
-// Measured at 24 rows on 16 experts, 512 -> 2048 (31.7 MB): 8.8 us, 19.1 with the pair kernel.
+// Measured at 24 rows on 16 experts, 512 -> 2048 (31.7 MB): 8.8 us, 19.1 with the pair kernel.  What decides between the two stands
+// in ragged.cu.  The second kernel makes weight gradients in tiles of the same size.
 // Every wait is bounded; one that gives up raises the status word and the roles drain through the barriers.
 #include "ragged.cuh"
 
@@ -523,8 +524,9 @@ ragged_few_weights_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __g
                     float4 sum = v[b][0];
 #pragma unroll
                     for (int k = 1; k < SPLIT; ++k) sum = make_float4(sum.x + v[b][k].x, sum.y + v[b][k].y, sum.z + v[b][k].z, sum.w + v[b][k].w);
-                    __align__(8) const T out[4] = {from_float<T>(sum.x), from_float<T>(sum.y), from_float<T>(sum.z), from_float<T>(sum.w)};
-                    if (live[b]) *reinterpret_cast<uint2*>(static_cast<T*>(g.out) + (static_cast<int64_t>(e) * g.n + a0 + r[b]) * g.cols + b0 + c[b]) = *reinterpret_cast<const uint2*>(out);
+                    __align__(8) const T four[4] = {from_float<T>(sum.x), from_float<T>(sum.y), from_float<T>(sum.z), from_float<T>(sum.w)};
+                    T* dst = static_cast<T*>(g.out) + (static_cast<int64_t>(e) * g.n + a0 + r[b]) * g.cols + b0 + c[b];
+                    if (live[b]) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(four);
                 }
             }
             if (g.db != nullptr && rank == 0 && b0 == 0 && t < kTile && a0 + t < g.n) {
@@ -609,7 +611,8 @@ int launch(const CUtensorMap& tx, const CUtensorMap& tw, const RaggedArgs& g, in
                              static_cast<int>(kRingBytes + 1024 + (kMaxExperts + 1) * 8));
         attr_set[dev.index] = true;
     }
-    return launch_clusters(ragged_few_kernel<T, ROWS, GRADS, SPLIT>, SPLIT, ctas, kThreads, kRingBytes + 1024 + (static_cast<size_t>(g.experts) + 1) * 8, st, tx, tw, g);
+    return launch_clusters(ragged_few_kernel<T, ROWS, GRADS, SPLIT>, SPLIT, ctas, kThreads,
+                           kRingBytes + 1024 + (static_cast<size_t>(g.experts) + 1) * 8, st, tx, tw, g);
 }
 
 template <typename T, int ROWS, bool GRADS>
