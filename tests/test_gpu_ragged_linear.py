@@ -371,6 +371,30 @@ def test_weight_gradients_in_parts(sizes, n, k, dtype):
         assert torch.equal(dw, again[1]) and (not biased or torch.equal(db, again[2]))
 
 
+def test_parts_on_two_streams_and_in_a_graph():
+    """Clusters, pairs and single CTAs, each with tensor memory of its own, beside one another on two streams and captured."""
+    cases = [_case(sizes, n, k, torch.bfloat16, 60 + i) for i, (sizes, n, k) in enumerate([([3000], 128, 256), ([700] * 20, 512, 512), ([20000, 9000], 256, 256), ([9] * 30, 264, 520)])]
+    run = lambda: [ops.ragged_linear_backward(x, w, off, dy, bias=True) for x, w, off, dy, _bias, _ends in cases]
+    want = run()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    results = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s, out in zip(streams, results):
+            with torch.cuda.stream(s):
+                out.append(run())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = run()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for got in results[0] + results[1] + [captured]:
+        assert all(torch.equal(a, b) for case, right in zip(got, want) for a, b in zip(case, right))
+
+
 EDGES = [1, 0, 31, 32, 33, 127, 128, 129, 255, 256, 257, 1500, 900]
 
 
