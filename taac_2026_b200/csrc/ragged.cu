@@ -895,9 +895,9 @@ constexpr int64_t kShareRows = 2 * kSnap * kBlock;
 // bias gradient, in us: 16 experts of 128 rows, 512 -> 2048, 15.8 / 20.4, of 512 29.1 / 30.0, of 1024 49.6 / 46.5; 256 of 128 rows, 512 -> 512,
 // 48 / 61; one of 1000, 512 -> 512, 10.2 / 21.0, of 8000 17.5 / 27.0, of 60000 75.6 / 54.2; 20 of 1500, 256 -> 256, 17.2 / 25.3; 2 of 3000,
 // 512 -> 2048, 24.9 / 33.1; 4 of 10000, 1024 -> 1024, 132.8 / 108.8; one of 100000, 128 -> 128, 102.9 / 58.5.
-bool few_weights(const RaggedArgs& g) {
-    const auto tiles = [&](int tile) { return static_cast<int64_t>(g.experts) * ((g.n + tile - 1) / tile) * ((g.cols + tile - 1) / tile); };
-    const int64_t blocks = (g.T / g.experts + kBlock - 1) / kBlock, small = tiles(128), large = tiles(kTile), pairs = pairs_here(), here = 4 * pairs;
+bool few_weights(int32_t experts, int64_t T, int32_t N, int32_t K) {
+    const auto tiles = [&](int tile) { return static_cast<int64_t>(experts) * ((N + tile - 1) / tile) * ((K + tile - 1) / tile); };
+    const int64_t blocks = (T / experts + kBlock - 1) / kBlock, small = tiles(128), large = tiles(kTile), pairs = pairs_here(), here = 4 * pairs;
     const int64_t split = weights_split(small, blocks, here), part = (blocks + split - 1) / split;
     const int64_t few = (split > 1 ? 900 : 600) + 65 * ((small * split + here - 1) / here) * (part > 5 ? part : 5);
     const int64_t length = blocks > 7 ? blocks : 7;
@@ -908,7 +908,7 @@ bool few_weights(const RaggedArgs& g) {
 
 template <typename T>
 int weights_of(const void* x, const void* dy, RaggedArgs g, cudaStream_t st) {
-    if (few_weights(g)) return ragged_few_weights(x, dy, g, std::is_same<T, __nv_bfloat16>::value, st);
+    if (few_weights(g.experts, g.T, g.n, g.cols)) return ragged_few_weights(x, dy, g, std::is_same<T, __nv_bfloat16>::value, st);
     CUtensorMap ta, tb, to;
     const uint64_t rows = static_cast<uint64_t>(g.T);
     const bool chunked = g.n % 64 == 0 && g.cols % 64 == 0;
@@ -923,8 +923,10 @@ int weights_of(const void* x, const void* dy, RaggedArgs g, cudaStream_t st) {
     return launch_status();
 }
 
-// floats of the workspace for shared tiles: their descriptions and the partial tiles
-int64_t share_floats(int64_t T) { return T >= kShareRows ? static_cast<int64_t>(pairs_here()) * (8 + 2 * kTile + 2 * kPartFloats) : 0; }
+// floats of the workspace for shared tiles, where the pairs make the weight gradients: their descriptions and the partial tiles
+int64_t share_floats(int32_t experts, int64_t T, int32_t N, int32_t K) {
+    return T < kShareRows || few_weights(experts, T, N, K) ? 0 : static_cast<int64_t>(pairs_here()) * (8 + 2 * kTile + 2 * kPartFloats);
+}
 
 // How the sum of the bias gradient's rows is laid over the chip: as many threads along the columns as there are octets (whole warps, at
 // most the CTA), the others along the rows; four CTAs an SM, at least 16 rows each
@@ -999,8 +1001,8 @@ extern "C" int tb200_ragged_gemm_dgrad(const void* dy, const void* w, const int3
 
 extern "C" int64_t tb200_ragged_wgrad_workspace_bytes(int32_t experts, int64_t T, int32_t N, int32_t K) {
     using namespace tb200;
-    if (checked(experts, T, N, K, TB200_BF16) != TB200_OK || experts == 0) return 0;
-    return 4 * (share_floats(T) + (bias_shape(T, N).chunks + experts) * N);
+    if (checked(experts, T, N, K, TB200_BF16) != TB200_OK || experts == 0 || !device_info().valid) return 0;
+    return 4 * (share_floats(experts, T, N, K) + (bias_shape(T, N).chunks + experts) * N);
 }
 
 extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int32_t* offsets, void* dw, float* db, float* workspace, int32_t experts,
@@ -1028,7 +1030,8 @@ extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int3
     g.T = T;
     g.cols = K;
     g.n = N;
-    if (T >= kShareRows) {
+    const int64_t shared = share_floats(experts, T, N, K);
+    if (shared > 0) {
         g.pieces = reinterpret_cast<int4*>(workspace);
         g.db_partial = workspace + pairs_here() * 8;
         g.partial = g.db_partial + pairs_here() * 2 * kTile;
@@ -1037,7 +1040,7 @@ extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int3
         g.db = db;
         return dtype == TB200_BF16 ? weights_of<__nv_bfloat16>(x, dy, g, st) : weights_of<__half>(x, dy, g, st);
     }
-    float* part = workspace + share_floats(T);
+    float* part = workspace + shared;
     const BiasShape b = bias_shape(T, N);
     const dim3 grid(static_cast<unsigned>(b.chunks), b.columns), block(b.tx, 256 / b.tx);
     const size_t rows = (static_cast<size_t>(experts) + 1) * 4, smem = static_cast<size_t>(256 / b.tx - 1) * b.tx * 8 * 4 + rows;

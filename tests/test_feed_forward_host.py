@@ -150,3 +150,6 @@ def test_ragged_entries(lib):
     assert wgrad(P(p), P(p), P(p), P(p), None, None, 2, 4, 64, 64, BF16, None, None) == ERR_NULL
     assert wgrad(None, P(p), P(p), P(p), None, P(p), 2, 4, 64, 64, BF16, None, None) == ERR_NULL
     assert wgrad(P(p), P(p), P(p), P(p), P(p + 4), P(p), 2, 4, 64, 64, BF16, None, None) == ERR_ALIGN
+    size = lib.tb200_ragged_wgrad_workspace_bytes
+    assert size(0, 4, 64, 64) == 0 and size(2, -1, 64, 64) == 0 and size(2, 4, 12, 64) == 0
+    assert size(1, 100000, 512, 512) >= 0 and size(8, 4096, 512, 512) >= 0          # without a device too

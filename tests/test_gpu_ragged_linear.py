@@ -371,6 +371,13 @@ def test_weight_gradients_in_parts(sizes, n, k, dtype):
         assert torch.equal(dw, again[1]) and (not biased or torch.equal(db, again[2]))
 
 
+def test_workspace_for_partial_tiles_only_where_pairs_share_them():
+    from taac_2026_b200 import _lib
+
+    size = _lib.load().tb200_ragged_wgrad_workspace_bytes
+    assert size(8, 4096, 512, 512) < 1 << 23 <= size(1, 200000, 512, 512)
+
+
 def test_parts_on_two_streams_and_in_a_graph():
     """Clusters, pairs and single CTAs, each with tensor memory of its own, beside one another on two streams and captured."""
     cases = [_case(sizes, n, k, torch.bfloat16, 60 + i) for i, (sizes, n, k) in enumerate([([3000], 128, 256), ([700] * 20, 512, 512), ([20000, 9000], 256, 256), ([9] * 30, 264, 520)])]
