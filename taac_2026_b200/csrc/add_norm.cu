@@ -62,6 +62,24 @@ struct FwdArgs {
     float eps;
 };
 
+// Between these the quotient 448 / amax and its quick form are accurate: a divisor above 2^126 gives the quick form 0, and below
+// 448 / 2^128 the quotient is infinite, though amax / 448 is a number at both ends.
+constexpr float kLeastAmax = 0x1p-100f, kMostAmax = 0x1p100f;
+
+// The factor of a block outside of them, which takes n by 2^+-100 nearer to 1 first (exact, but for values that are nothing beside the
+// block's largest).  It is the reciprocal of the scale as it is stored, which has few bits where it is subnormal.  A scale that
+// rounds to zero becomes 1: the block's values, below 2^-141, are zeros.  Infinity makes the whole block NaN.
+__device__ __forceinline__ float far_factor(float amax, float* scale, float2 (&n)[4]) {
+    if (!(*scale > 0.f)) {
+        *scale = 1.0f;
+        return 1.0f;
+    }
+    const float nearer = amax > 1.0f ? 0x1p-100f : 0x1p100f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) n[e] = __fmul2_rn(n[e], make_float2(nearer, nearer));
+    return __fdividef(1.0f, *scale * nearer);
+}
+
 // OPT: octets of a lane; G: see row_sum; SC: kind of scales
 template <typename T, int OPT, int G, int SC>
 __global__ void __launch_bounds__(G == 0 ? kMaxWideThreads : kThreads)
@@ -143,9 +161,10 @@ add_norm_kernel(const FwdArgs<T> a) {
                 uint32_t byte = 0;
                 if (SC == kAmax) {                           // the rule of tb200_quant_act_1x128, on the unrounded n
                     // the product and the quick quotient are within 2^-22: every lane forms them, a division would cost a quarter
-                    // of the kernel's instructions.  A block of subnormal values keeps a finite factor, for its zeros.
-                    scale = amax > 0.f ? amax * (1.0f / 448.0f) : 1.0f;
-                    inv = amax > 0.f ? fminf(__fdividef(448.0f, amax), 3.0e38f) : 1.0f;
+                    // of the kernel's instructions.
+                    scale = amax * (1.0f / 448.0f);
+                    inv = __fdividef(448.0f, amax);
+                    if (!(amax >= kLeastAmax && amax <= kMostAmax)) inv = far_factor(amax, &scale, t[j]);      // the block's 16 lanes alike
                 } else {
                     byte = pow2_scale(amax, &inv);
                 }
