@@ -1,4 +1,5 @@
-"""`add_rms_norm_quant` at the ends of its range: blocks whose largest value lies anywhere in fp32.
+"""`add_rms_norm_quant` and `add_rms_norm_backward` at the ends of their range: blocks whose largest value lies anywhere in fp32, and
+eps = 0 where lanes of a warp have no row.
 
 Tolerances as in test_gpu_add_norm.py: F32 for the fp32 steps in front of a stored value, half an e4m3 step for q.  Next to fp32's
 subnormal numbers the value and its block's scale are each off by up to half a step of 2^-149, the scale's counted up to 448 times."""
@@ -69,3 +70,23 @@ def test_blocks_of_different_magnitude_in_a_row():
     n = xd * torch.rsqrt(xd.pow(2).mean(-1, keepdim=True) + 1e-6) * weight.double()
     wide = sc.double().repeat_interleave(128, -1)
     _within(q.double() * wide, n, torch.maximum(2.0 ** -4 * n.abs(), 2.0 ** -10 * wide) * (1 + 1e-5) + 450 * STEP)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("cols", [8, 64, 128, 256, 1024])
+@pytest.mark.parametrize("rows", [1, 2, 15, 17, 301])
+def test_gradient_of_the_weight_without_eps(dtype, cols, rows):
+    """A row of 16 lanes shares its warp with another, which has none where the number of rows is odd."""
+    g = torch.Generator(device="cuda").manual_seed(rows * 1000 + cols)
+    t, dn = (torch.randn(rows, cols, generator=g, device="cuda").to(dtype) for _ in range(2))
+    w = torch.ones(cols, device="cuda", dtype=dtype)
+    grad, dw = ops.add_rms_norm_backward(t, w, dn, None, eps=0.0)
+    td, gd = t.double(), dn.double()
+    s = torch.rsqrt(td.pow(2).mean(-1, keepdim=True))
+    xh = td * s
+    half, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    m = (gd * xh).mean(-1, keepdim=True)
+    want = s * (gd - xh * m)
+    _within(grad, want, half * want.abs() + 2 * F32 * s * (gd.abs() + xh.abs() * (gd * xh).abs().mean(-1, keepdim=True)) + tiny)
+    terms = gd * xh
+    _within(dw, terms.sum(0), half * terms.sum(0).abs() + ((rows / 296 + 64) * 2.0 ** -24 + F32) * terms.abs().sum(0) + tiny)
