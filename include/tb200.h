@@ -149,7 +149,8 @@ int tb200_add_rmsnorm_bwd(const void* total, const void* gamma, const void* d_no
 
 /* Activations kept in 8 bits for the backward pass: q e4m3 [rows, cols], scales fp32 [rows, cols / 128] = the smallest
  * power of two s with max|x| / s <= 448 over the finite values of the block; values that are not finite are kept as NaN.
- * x / s and q s are exact.  cols % 128 == 0. */
+ * x / s and q s are exact.  A finite q s that the type of a restored value (or of h below) does not hold becomes the type's
+ * largest number: fp16 values from 63488 on are kept as 65536 and come back as 65504.  cols % 128 == 0. */
 int tb200_keep_fwd(const void* x, void* q, float* scales, int64_t rows, int32_t cols, int dtype, void* stream);
 int tb200_keep_restore(const void* q, const float* scales, void* x, int64_t rows, int32_t cols, int dtype, void* stream);
 /* The activation of a feed-forward layer: h [rows, hidden] = silu(gate) * value of up [rows, 2 hidden] = [gate | value]

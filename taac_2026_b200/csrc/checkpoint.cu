@@ -4,10 +4,13 @@
 //             q = e4m3(x / s).  Both divisions and q s are exact, so that what was kept is restored without a second
 //             rounding (bf16 and fp32; fp16 where the value is in its range), and a kernel that computes from q sees the
 //             values that any other reader of the checkpoint sees.  Infinities and NaN are kept as NaN and leave the
-//             scale of their block alone, so that a gradient computed from them does not look finite.
+//             scale of their block alone, so that a gradient computed from them does not look finite.  Finite values stay
+//             finite: those from 31 / 32 of the power of two behind their type's range on are kept as that power of two, and a
+//             reader whose type does not hold a value takes its largest number.
 //   silu_gate h = g sig(g) v          (gated: up = [g | v] or [v | g])      h = g sig(g)     (not gated)
 //   backward  dv = dh g sig(g),  dg = dh v sig(g) (1 + g (1 - sig(g))), and h once more: the next layer's weight
-//             gradient needs it, and it comes from the same 8 bits instead of 16 kept ones.
+//             gradient needs it, and it comes from the same 8 bits instead of 16 kept ones (its type's largest number where
+//             the kept values' rounding took it behind that).
 //
 // Bound by HBM: each value is read and written once.  A lane works on an octet (8 columns), 16 neighbouring lanes hold a
 // block of 128 columns, whose largest value is found by four shuffles; a lane has kUnroll octets of different places in
@@ -35,6 +38,42 @@ __device__ __forceinline__ float sigmoid(float g) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-g)));
     return r;
+}
+
+// Finite numbers that a type does not hold become its largest one, two packed values at a time behind their rounding (infinity is what
+// they round to there); NaN stays NaN.  The sign is the value's, the limit being positive.
+template <typename T>
+__device__ __forceinline__ uint32_t held(uint32_t x) {
+    uint32_t y;
+    if (std::is_same<T, __half>::value) asm("min.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x7BFF7BFFu));
+    else if (sizeof(T) == 2) asm("min.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x7F7F7F7Fu));
+    else asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x7F7FFFFFu));
+    return y;
+}
+template <typename T>
+__device__ __forceinline__ void store_held(T* p, const float2 (&f)[4]) {
+    constexpr int N = Vec16<T>::N / 2;
+#pragma unroll
+    for (int i = 0; i < Octet<T>::P; ++i) {
+        float2 g[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) g[e] = f[i * N + e];
+        const uint4 w = Vec16<T>::pack2(g);
+        *(reinterpret_cast<uint4*>(p) + i) = make_uint4(held<T>(w.x), held<T>(w.y), held<T>(w.z), held<T>(w.w));
+    }
+}
+
+// The values that eight e4m3 bytes stand for.  From s = 2^120 on they may be infinite where the bytes are not: see finite.
+__device__ __forceinline__ void kept_values(uint2 q, float s, float2 (&x)[4]) {
+    unpack_e4m3x8(q, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __fmul2_rn(x[e], make_float2(s, s));
+}
+__device__ __forceinline__ bool huge_scale(float s) { return s > 0x1p119f; }
+__device__ __forceinline__ void finite(float2 (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        x[e] = make_float2(__uint_as_float(held<float>(__float_as_uint(x[e].x))), __uint_as_float(held<float>(__float_as_uint(x[e].y))));
 }
 
 // ---- largest value of a block.  |x| of every type orders as its bits do, infinity and NaN on top, so the maximum is taken of
@@ -190,9 +229,10 @@ gate_kernel(const T* __restrict__ up, T* __restrict__ h, uint2* __restrict__ q, 
     }
 }
 
-// MODE: 0 restore (q, scales -> x), 1 backward of the ungated form, 2 of the gated one
+// MODE: 0 restore (q, scales -> x), 1 backward of the ungated form, 2 of the gated one.  16-bit types: four CTAs an SM (left alone the
+// gated form takes 66 registers, three CTAs: 32768 x 2048 119 us a call instead of 109)
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, MODE == 2 && sizeof(T) == 2 ? 4 : 0)
 gate_bwd_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, const T* __restrict__ dh, T* __restrict__ dup, T* __restrict__ h,
                 uint32_t items, uint32_t octets, int32_t gate_at) {
     chain_release();
@@ -226,18 +266,17 @@ gate_bwd_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, c
         for (int u = 0; u < kUnroll; ++u) {
             if (base + u * stride >= items) continue;
             float2 g[4], v[4], d[4], o[4];
-            unpack_e4m3x8(qg[u], g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) g[e] = __fmul2_rn(g[e], make_float2(sg[u], sg[u]));
+            kept_values(qg[u], sg[u], g);
             const int64_t ig = (in[u] + to_gate) * 8;
             if (MODE == 0) {
-                Octet<T>::store2(dup + ig, g);
+                if (huge_scale(sg[u])) finite(g);
+                store_held(dup + ig, g);
                 continue;
             }
-            if (MODE == 2) {
-                unpack_e4m3x8(qv[u], v);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(v[e], make_float2(sv[u], sv[u]));
+            if (MODE == 2) kept_values(qv[u], sv[u], v);
+            if (huge_scale(MODE == 2 ? fmaxf(sg[u], sv[u]) : sg[u])) {      // a branch for both: one for each takes 1 % more
+                finite(g);
+                if (MODE == 2) finite(v);
             }
             rd[u].unpack2(d);
             const float2 one = make_float2(1.f, 1.f);
@@ -259,7 +298,7 @@ gate_bwd_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, c
             }
             Octet<T>::store2(dup + ig, d);
             if (MODE == 2) Octet<T>::store2(dup + (in[u] + to_value) * 8, g);
-            if (h != nullptr) Octet<T>::store2(h + static_cast<int64_t>(base + u * stride) * 8, o);
+            if (h != nullptr) store_held(h + static_cast<int64_t>(base + u * stride) * 8, o);
         }
     }
 }

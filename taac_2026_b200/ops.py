@@ -1597,7 +1597,8 @@ def checkpoint_activation(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def restore_activation(q: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values that ``checkpoint_activation`` kept, ``q * scale``, in ``dtype`` (exact in fp32 and bf16, and in fp16 in its range)."""
+    """The values that ``checkpoint_activation`` kept, ``q * scale``, in ``dtype``: exact in fp32 and bf16, and in fp16 in its range.
+    A finite one that ``dtype`` does not hold becomes its largest number (fp16: 65504 for values kept from 63488 on)."""
     if dtype not in _DTYPE_CODES:
         raise ValueError(f"restore_activation does not support dtype {dtype}")
     matrix, s = _kept_operand("restore_activation", q, scales)
@@ -1652,7 +1653,8 @@ def silu_gate_backward(q: torch.Tensor, scales: torch.Tensor, grad: torch.Tensor
                        activation: bool = True) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(grad_up, h): the gradient of ``silu_gate``'s input from what ``silu_gate_checkpoint`` kept and the gradient of its
     result, and (``activation=True``) the activation of the kept values: the weight gradient of the layer behind it needs
-    it, and so nothing else has to be kept for that.  Both in ``grad``'s dtype."""
+    it, and so nothing else has to be kept for that (held at its type's largest number where the rounding to 8 bits took a product
+    behind it).  Both in ``grad``'s dtype."""
     if _TIMING is None:
         fast = _host.silu_gate_backward(q, scales, grad, gated, gate_first, activation)
         if fast is not None:
