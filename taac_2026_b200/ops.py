@@ -1796,7 +1796,7 @@ def ragged_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, 
 
     Differentiable in x, weight, bias and residual (without ``silu`` and ``out``).  ``checkpoint=True`` keeps x for the
     weight gradient in 8 bits (``checkpoint_activation``; K a multiple of 128) instead of as it is.  ``check`` / ``status``: as
-    in ``grouped_linear``."""
+    in ``grouped_linear``, for the backward pass too."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         if silu or out is not None:
             raise RuntimeError("cuda ragged_linear is forward-only with silu or out: use silu_gate(gated=False) behind it for training")
@@ -1889,6 +1889,7 @@ class _RaggedLinearFunction(torch.autograd.Function):
         ctx.save_for_backward(kept, scales, weight, offsets)
         ctx.rows = x.shape
         ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.check, ctx.status = check, status
         with torch.no_grad():
             return ragged_linear(x, weight, offsets, bias, residual=residual, check=check, status=status)
 
@@ -1898,7 +1899,8 @@ class _RaggedLinearFunction(torch.autograd.Function):
         kept, scales, weight, offsets = ctx.saved_tensors
         need_x, need_w, _o, need_b, need_r = ctx.needs_input_grad[:5]
         x = kept if kept is not None else grad_out.new_empty(1).expand(ctx.rows)     # its shape alone is read
-        dx, dw, db = ragged_linear_backward(x, weight, offsets, grad_out, scales=scales, bias=need_b, need_x=need_x, need_weight=need_w)
+        dx, dw, db = ragged_linear_backward(x, weight, offsets, grad_out, scales=scales, bias=need_b, need_x=need_x, need_weight=need_w,
+                                            check=ctx.check, status=ctx.status)
         return dx, dw, None, None if db is None else db.to(ctx.bias_dtype), grad_out if need_r else None, None, None, None
 
 

@@ -511,3 +511,14 @@ def test_served_in_8_bits():
 
 def _norm64(t):
     return t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + 1e-6)
+
+
+def test_status_word_under_autograd():
+    """The caller's word and check=True serve the backward pass as well, with the same gradients."""
+    x, w, off, dy, bias, _ends = _case([700, 0, 300], 264, 136, torch.bfloat16, 61)
+    want = ops.ragged_linear_backward(x, w, off, dy, bias=True)
+    word = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for kw in ({"status": word}, {"check": True}, {"status": word, "check": True}):
+        leaves = [t.clone().requires_grad_() for t in (x, w, bias)]
+        ops.ragged_linear(leaves[0], leaves[1], off, leaves[2], **kw).backward(dy)
+        assert all(torch.equal(leaf.grad, v) for leaf, v in zip(leaves, want)) and int(word) == 0
