@@ -160,7 +160,7 @@ int tb200_keep_restore(const void* q, const float* scales, void* x, int64_t rows
 int tb200_silu_gate_fwd(const void* up, void* h, void* q, float* scales, int64_t rows, int32_t hidden, int32_t gated,
                         int32_t gate_first, int dtype, void* stream);
 /* Its gradient dup from the kept values and dh; h (may be NULL) receives the activation again, for the weight gradient of
- * the layer behind it.  dtype: of dh, dup and h. */
+ * the layer behind it.  dtype: of dh, dup and h.  scales NULL: q is `up` itself, of that dtype. */
 int tb200_silu_gate_bwd(const void* q, const float* scales, const void* dh, void* dup, void* h, int64_t rows, int32_t hidden,
                         int32_t gated, int32_t gate_first, int dtype, void* stream);
 

@@ -10,7 +10,8 @@
 //   silu_gate h = g sig(g) v          (gated: up = [g | v] or [v | g])      h = g sig(g)     (not gated)
 //   backward  dv = dh g sig(g),  dg = dh v sig(g) (1 + g (1 - sig(g))), and h once more: the next layer's weight
 //             gradient needs it, and it comes from the same 8 bits instead of 16 kept ones (its type's largest number where
-//             the kept values' rounding took it behind that).
+//             the kept values' rounding took it behind that).  The same from the input itself, for a gradient that 8 bits
+//             do not round.
 //
 // Bound by HBM: each value is read and written once.  A lane works on an octet (8 columns), 16 neighbouring lanes hold a
 // block of 128 columns, whose largest value is found by four shuffles; a lane has kUnroll octets of different places in
@@ -229,11 +230,30 @@ gate_kernel(const T* __restrict__ up, T* __restrict__ h, uint2* __restrict__ q, 
     }
 }
 
-// MODE: 0 restore (q, scales -> x), 1 backward of the ungated form, 2 of the gated one.  16-bit types: four CTAs an SM (left alone the
+// What the backward pass computes from: eight kept values with their scale, or eight of the input itself (T)
+template <typename T, bool KEPT>
+struct Source {
+    uint2 q;
+    float s;
+    __device__ void load(const void* from, const float* scales, int64_t at) {
+        q = __ldcs(static_cast<const uint2*>(from) + at);
+        s = __ldg(scales + (at >> 4));
+    }
+    __device__ void values(float2 (&x)[4]) const { kept_values(q, s, x); }
+};
+template <typename T>
+struct Source<T, false> {
+    Octet<T> v;
+    static constexpr float s = 1.0f;
+    __device__ void load(const void* from, const float*, int64_t at) { v.load(static_cast<const T*>(from) + at * 8); }
+    __device__ void values(float2 (&x)[4]) const { v.unpack2(x); }
+};
+
+// MODE: 0 restore (q, scales -> x), 1 backward of the ungated form, 2 of the gated one.  KEPT: `from` holds e4m3 values, else T.  16-bit types: four CTAs an SM (left alone the
 // gated form takes 66 registers, three CTAs: 32768 x 2048 119 us a call instead of 109)
-template <typename T, int MODE>
+template <typename T, int MODE, bool KEPT>
 __global__ void __launch_bounds__(kThreads, MODE == 2 && sizeof(T) == 2 ? 4 : 0)
-gate_bwd_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, const T* __restrict__ dh, T* __restrict__ dup, T* __restrict__ h,
+gate_bwd_kernel(const void* __restrict__ from, const float* __restrict__ scales, const T* __restrict__ dh, T* __restrict__ dup, T* __restrict__ h,
                 uint32_t items, uint32_t octets, int32_t gate_at) {
     chain_release();
     chain_wait();
@@ -243,21 +263,15 @@ gate_bwd_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, c
     const Place by(stride, octets);
     Place place(blockIdx.x * kThreads + threadIdx.x, octets);
     for (uint32_t base = blockIdx.x * kThreads + threadIdx.x; base < items; base += kUnroll * stride) {
-        uint2 qg[kUnroll], qv[kUnroll];
-        float sg[kUnroll], sv[kUnroll];
+        Source<T, KEPT> sg[kUnroll], sv[kUnroll];
         Octet<T> rd[kUnroll];
         int64_t in[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             in[u] = static_cast<int64_t>(place.row) * width + place.col;
             if (base + u * stride < items) {
-                const int64_t ig = in[u] + to_gate, iv = in[u] + to_value;
-                qg[u] = __ldcs(q + ig);
-                sg[u] = __ldg(scales + (ig >> 4));
-                if (MODE == 2) {
-                    qv[u] = __ldcs(q + iv);
-                    sv[u] = __ldg(scales + (iv >> 4));
-                }
+                sg[u].load(from, scales, in[u] + to_gate);
+                if (MODE == 2) sv[u].load(from, scales, in[u] + to_value);
                 if (MODE != 0) rd[u].load(dh + static_cast<int64_t>(base + u * stride) * 8);
             }
             place.advance(by, octets);
@@ -266,15 +280,15 @@ gate_bwd_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, c
         for (int u = 0; u < kUnroll; ++u) {
             if (base + u * stride >= items) continue;
             float2 g[4], v[4], d[4], o[4];
-            kept_values(qg[u], sg[u], g);
+            sg[u].values(g);
             const int64_t ig = (in[u] + to_gate) * 8;
             if (MODE == 0) {
-                if (huge_scale(sg[u])) finite(g);
+                if (huge_scale(sg[u].s)) finite(g);
                 store_held(dup + ig, g);
                 continue;
             }
-            if (MODE == 2) kept_values(qv[u], sv[u], v);
-            if (huge_scale(MODE == 2 ? fmaxf(sg[u], sv[u]) : sg[u])) {      // a branch for both: one for each takes 1 % more
+            if (MODE == 2) sv[u].values(v);
+            if (KEPT && huge_scale(MODE == 2 ? fmaxf(sg[u].s, sv[u].s) : sg[u].s)) {      // a branch for both: one for each takes 1 % more
                 finite(g);
                 if (MODE == 2) finite(v);
             }
@@ -298,7 +312,11 @@ gate_bwd_kernel(const uint2* __restrict__ q, const float* __restrict__ scales, c
             }
             Octet<T>::store2(dup + ig, d);
             if (MODE == 2) Octet<T>::store2(dup + (in[u] + to_value) * 8, g);
-            if (h != nullptr) store_held(h + static_cast<int64_t>(base + u * stride) * 8, o);
+            if (h != nullptr) {      // from the input itself it is the forward pass's, which held nothing
+                T* at = h + static_cast<int64_t>(base + u * stride) * 8;
+                if (KEPT) store_held(at, o);
+                else Octet<T>::store2(at, o);
+            }
         }
     }
 }
@@ -330,15 +348,16 @@ int run_gate(const void* up, void* h, void* q, float* scales, int64_t rows, int3
     return TB200_OK;
 }
 
-template <typename T, int MODE>
-int run_gate_bwd(const void* q, const float* scales, const void* dh, void* dup, void* h, int64_t rows, int32_t hidden, int gate_at,
+template <typename T, int MODE, bool KEPT>
+int run_gate_bwd(const void* from, const float* scales, const void* dh, void* dup, void* h, int64_t rows, int32_t hidden, int gate_at,
                  cudaStream_t st) {
     const int64_t octets = hidden / 8, width = octets * (MODE == 2 ? 2 : 1);
     const int64_t chunk = kMaxItems / octets;
     for (int64_t r = 0; r < rows; r += chunk) {
         const int64_t n = rows - r < chunk ? rows - r : chunk;
-        launch_chained(gate_bwd_kernel<T, MODE>, grid_of(n * octets, 64), kThreads, 0, st, static_cast<const uint2*>(q) + r * width,
-                       scales + r * width / 16, MODE == 0 ? nullptr : static_cast<const T*>(dh) + r * hidden,
+        launch_chained(gate_bwd_kernel<T, MODE, KEPT>, grid_of(n * octets, 64), kThreads, 0, st,
+                       static_cast<const void*>(static_cast<const uint8_t*>(from) + r * width * 8 * (KEPT ? 1 : sizeof(T))),
+                       KEPT ? scales + r * width / 16 : nullptr, MODE == 0 ? nullptr : static_cast<const T*>(dh) + r * hidden,
                        static_cast<T*>(dup) + r * width * 8, h == nullptr ? nullptr : static_cast<T*>(h) + r * hidden,
                        static_cast<uint32_t>(n * octets), static_cast<uint32_t>(octets), gate_at);
         count_launch();
@@ -366,7 +385,10 @@ int gate_of(const void* up, void* h, void* q, float* scales, int64_t rows, int32
 template <typename T>
 int gate_bwd_of(const void* q, const float* scales, const void* dh, void* dup, void* h, int64_t rows, int32_t hidden, int gated, int gate_at,
                 cudaStream_t st) {
-    return gated ? run_gate_bwd<T, 2>(q, scales, dh, dup, h, rows, hidden, gate_at, st) : run_gate_bwd<T, 1>(q, scales, dh, dup, h, rows, hidden, 0, st);
+    if (scales == nullptr)
+        return gated ? run_gate_bwd<T, 2, false>(q, scales, dh, dup, h, rows, hidden, gate_at, st)
+                     : run_gate_bwd<T, 1, false>(q, scales, dh, dup, h, rows, hidden, 0, st);
+    return gated ? run_gate_bwd<T, 2, true>(q, scales, dh, dup, h, rows, hidden, gate_at, st) : run_gate_bwd<T, 1, true>(q, scales, dh, dup, h, rows, hidden, 0, st);
 }
 
 }  // namespace
@@ -396,9 +418,9 @@ extern "C" int tb200_keep_restore(const void* q, const float* scales, void* x, i
     if (!device_info().valid) return TB200_ERR_DEVICE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case TB200_F32: return run_gate_bwd<float, 0>(q, scales, nullptr, x, nullptr, rows, cols, 0, st);
-        case TB200_F16: return run_gate_bwd<__half, 0>(q, scales, nullptr, x, nullptr, rows, cols, 0, st);
-        default: return run_gate_bwd<__nv_bfloat16, 0>(q, scales, nullptr, x, nullptr, rows, cols, 0, st);
+        case TB200_F32: return run_gate_bwd<float, 0, true>(q, scales, nullptr, x, nullptr, rows, cols, 0, st);
+        case TB200_F16: return run_gate_bwd<__half, 0, true>(q, scales, nullptr, x, nullptr, rows, cols, 0, st);
+        default: return run_gate_bwd<__nv_bfloat16, 0, true>(q, scales, nullptr, x, nullptr, rows, cols, 0, st);
     }
 }
 
@@ -424,7 +446,7 @@ extern "C" int tb200_silu_gate_bwd(const void* q, const float* scales, const voi
     using namespace tb200;
     const int code = checked(rows, hidden, dtype);
     if (code != TB200_OK || rows == 0) return code;
-    if (q == nullptr || scales == nullptr || dh == nullptr || dup == nullptr) return TB200_ERR_NULL;
+    if (q == nullptr || dh == nullptr || dup == nullptr) return TB200_ERR_NULL;
     if (!aligned16(q) || !aligned16(dh) || !aligned16(dup) || !aligned16(h) || (reinterpret_cast<uintptr_t>(scales) & 3) != 0) return TB200_ERR_ALIGN;
     if (!device_info().valid) return TB200_ERR_DEVICE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -641,20 +641,22 @@ PyObject* py_silu_gate(PyObject*, PyObject* const* args, Py_ssize_t) {
     END_HANDLE_TH_ERRORS
 }
 
-// silu_gate_backward(q, scales, grad, gated, gate_first, activation) -> (grad_up, h or None)
+// silu_gate_backward(q, scales or None, grad, gated, gate_first, activation) -> (grad_up, h or None)
 PyObject* py_silu_gate_backward(PyObject*, PyObject* const* args, Py_ssize_t) {
     HANDLE_TH_ERRORS
-    if (!is_tensor(args[0]) || !is_tensor(args[1]) || !is_tensor(args[2])) Py_RETURN_NONE;
+    if (!is_tensor(args[0]) || !is_optional(args[1]) || !is_tensor(args[2])) Py_RETURN_NONE;
     const Tensor& q = tensor(args[0]);
-    const Tensor& scales = tensor(args[1]);
+    const auto scales = optional_tensor(args[1]);
     const Tensor& dh = tensor(args[2]);
     const bool gated = truth(args[3]), first = truth(args[4]), activation = truth(args[5]);
     const auto t = dh.scalar_type();
-    if (q.dim() < 1 || dtype_code(t) < 0 || !plain(q, at::kFloat8_e4m3fn, q) || !plain(dh, t, q) || !dense(scales, at::kFloat) ||
-        scales.device() != q.device() || q.numel() == 0 || q.size(-1) % (gated ? 256 : 128) != 0 || q.size(-1) > INT32_MAX)
+    if (q.dim() < 1 || dtype_code(t) < 0 || !plain(q, scales.has_value() ? at::kFloat8_e4m3fn : t, q) || !plain(dh, t, q) || q.numel() == 0 ||
+        q.size(-1) % (gated ? 256 : 128) != 0 || q.size(-1) > INT32_MAX)
         Py_RETURN_NONE;
     const int64_t width = q.size(-1), hidden = gated ? width / 2 : width, rows = q.numel() / width;
-    if (scales.sizes() != c10::IntArrayRef(sizes_with(q, width / 128)) || dh.sizes() != c10::IntArrayRef(sizes_with(q, hidden))) Py_RETURN_NONE;
+    if (scales.has_value() && (!dense(*scales, at::kFloat) || scales->device() != q.device() || scales->sizes() != c10::IntArrayRef(sizes_with(q, width / 128))))
+        Py_RETURN_NONE;
+    if (dh.sizes() != c10::IntArrayRef(sizes_with(q, hidden))) Py_RETURN_NONE;
     const c10::cuda::CUDAGuard guard(q.device());
     if (!tb200_device_ok()) Py_RETURN_NONE;
     const auto opt = dh.options().requires_grad(false);

@@ -1629,16 +1629,16 @@ def _silu_gate(up: torch.Tensor, gated: bool, gate_first: bool, keep: bool, name
     return (h, q.view(up.shape), scales.view(*up.shape[:-1], width // 128)) if keep else h
 
 
-def silu_gate(up: torch.Tensor, *, gated: bool = True, gate_first: bool = True, backend: str = "cuda") -> torch.Tensor:
+def silu_gate(up: torch.Tensor, *, gated: bool = True, gate_first: bool = True, checkpoint: bool = False, backend: str = "cuda") -> torch.Tensor:
     """The activation of a feed-forward layer: ``silu(gate) * value`` of ``up`` [..., 2 hidden] = [gate | value]
     (``gate_first``, experiments/tokenformer/model.py:118-128) or [value | gate] (experiments/baseline/model.py:99-113);
-    ``gated=False``: ``silu(up)`` (experiments/onetrans/model.py:33-44).
+    ``gated=False``: ``silu(up)`` (experiments/onetrans/model.py:33-44).  ``hidden`` is a multiple of 128.
 
-    Differentiable; what is kept for the backward pass is ``up`` in 8 bits (``silu_gate_checkpoint``), a rounding of half an
-    e4m3 step (2^-4) of each of its values that the gradient carries.  ``hidden`` is a multiple of 128."""
+    Differentiable.  ``checkpoint=True`` keeps ``up`` for the backward pass in 8 bits (``silu_gate_checkpoint``) instead of as it
+    is: a rounding of half an e4m3 step (2^-4) of each of its values that the gradient carries."""
     _require_backend_name("silu_gate", backend)
     if torch.is_grad_enabled() and up.requires_grad:
-        return _SiluGateFunction.apply(up, bool(gated), bool(gate_first))
+        return _SiluGateFunction.apply(up, bool(gated), bool(gate_first), bool(checkpoint))
     return _silu_gate(up, gated, gate_first, False, "silu_gate")
 
 
@@ -1649,17 +1649,22 @@ def silu_gate_checkpoint(up: torch.Tensor, *, gated: bool = True, gate_first: bo
     return _silu_gate(up, gated, gate_first, True, "silu_gate_checkpoint")
 
 
-def silu_gate_backward(q: torch.Tensor, scales: torch.Tensor, grad: torch.Tensor, *, gated: bool = True, gate_first: bool = True,
+def silu_gate_backward(q: torch.Tensor, scales: torch.Tensor | None, grad: torch.Tensor, *, gated: bool = True, gate_first: bool = True,
                        activation: bool = True) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(grad_up, h): the gradient of ``silu_gate``'s input from what ``silu_gate_checkpoint`` kept and the gradient of its
     result, and (``activation=True``) the activation of the kept values: the weight gradient of the layer behind it needs
     it, and so nothing else has to be kept for that (held at its type's largest number where the rounding to 8 bits took a product
-    behind it).  Both in ``grad``'s dtype."""
+    behind it).  Both in ``grad``'s dtype.  With ``scales=None`` q is the input itself, of ``grad``'s dtype."""
     if _TIMING is None:
         fast = _host.silu_gate_backward(q, scales, grad, gated, gate_first, activation)
         if fast is not None:
             return fast
-    matrix, s = _kept_operand("silu_gate_backward", q, scales, 2 if gated else 1)
+    if scales is None:
+        matrix, s = _keep_operand("silu_gate_backward", q, 2 if gated else 1), None
+        if grad.dtype != q.dtype:
+            raise ValueError(f"silu_gate_backward needs the input and grad of one dtype, got {q.dtype} and {grad.dtype}")
+    else:
+        matrix, s = _kept_operand("silu_gate_backward", q, scales, 2 if gated else 1)
     rows, width = matrix.shape
     hidden = width // 2 if gated else width
     if tuple(grad.shape) != (*q.shape[:-1], hidden):
@@ -1679,19 +1684,23 @@ def silu_gate_backward(q: torch.Tensor, scales: torch.Tensor, grad: torch.Tensor
 
 class _SiluGateFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, up, gated, gate_first):
+    def forward(ctx, up, gated, gate_first, checkpoint):
+        kept, scales = up, None
         with torch.no_grad():
-            h, q, scales = silu_gate_checkpoint(up, gated=gated, gate_first=gate_first)
-        ctx.save_for_backward(q, scales)
+            if checkpoint:
+                h, kept, scales = silu_gate_checkpoint(up, gated=gated, gate_first=gate_first)
+            else:
+                h = silu_gate(up, gated=gated, gate_first=gate_first)
+        ctx.save_for_backward(kept, scales)
         ctx.form = (gated, gate_first)
         return h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, scales = ctx.saved_tensors
+        kept, scales = ctx.saved_tensors
         gated, gate_first = ctx.form
-        return silu_gate_backward(q, scales, grad, gated=gated, gate_first=gate_first, activation=False)[0], None, None
+        return silu_gate_backward(kept, scales, grad, gated=gated, gate_first=gate_first, activation=False)[0], None, None, None
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, silu: bool = False,
