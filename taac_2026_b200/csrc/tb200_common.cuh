@@ -212,16 +212,6 @@ struct Octet {
 #pragma unroll
         for (int i = 0; i < P; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
     }
-    __device__ void unpack(float (&f)[8]) const {
-        constexpr int N = Vec16<T>::N;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            float g[N];
-            Vec16<T>::unpack(v[i], g);
-#pragma unroll
-            for (int e = 0; e < N; ++e) f[i * N + e] = g[e];
-        }
-    }
     __device__ void unpack2(float2 (&f)[4]) const {
         constexpr int N = Vec16<T>::N / 2;
 #pragma unroll
@@ -240,16 +230,6 @@ struct Octet {
 #pragma unroll
             for (int e = 0; e < N; ++e) g[e] = f[i * N + e];
             *(reinterpret_cast<uint4*>(p) + i) = Vec16<T>::pack2(g);
-        }
-    }
-    static __device__ void store(T* p, const float (&f)[8]) {
-        constexpr int N = Vec16<T>::N;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            float g[N];
-#pragma unroll
-            for (int e = 0; e < N; ++e) g[e] = f[i * N + e];
-            *(reinterpret_cast<uint4*>(p) + i) = Vec16<T>::pack(g);
         }
     }
 };
