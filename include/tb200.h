@@ -538,10 +538,11 @@ int tb200_ragged_gemm(const void* x, const void* w, const int32_t* offsets, cons
 int tb200_ragged_gemm_dgrad(const void* dy, const void* w, const int32_t* offsets, void* dx, int32_t experts, int64_t T, int32_t N,
                             int32_t K, int dtype, int32_t* status_word, void* stream);
 /* dw[e] = dy_e^T @ x_e ([experts, N, K], dtype) and db[e] = sum of the rows of dy_e (fp32 [experts, N]); either may be NULL (x
- * too without dw); zeros for an expert without rows.  Rows of no expert are not looked at.  workspace: device memory of
- * tb200_ragged_wgrad_workspace_bytes(...) bytes (on the current device; 0 without one), for this call alone.  The sums run in
- * a fixed order. */
+ * too without dw); zeros for an expert without rows.  Rows of no expert are not looked at.  workspace: device memory (never NULL,
+ * 0 bytes or not) for this call alone: tb200_ragged_wgrad_workspace_of bytes for calls with dw (weights = 1) or for those without (0),
+ * tb200_ragged_wgrad_workspace_bytes for both (on the current device; 0 without one).  The sums run in a fixed order. */
 int64_t tb200_ragged_wgrad_workspace_bytes(int32_t experts, int64_t T, int32_t N, int32_t K);
+int64_t tb200_ragged_wgrad_workspace_of(int32_t experts, int64_t T, int32_t N, int32_t K, int32_t weights);
 int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int32_t* offsets, void* dw, float* db, float* workspace,
                             int32_t experts, int64_t T, int32_t N, int32_t K, int dtype, int32_t* status_word, void* stream);
 

@@ -52,6 +52,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tb200_ragged_gemm": (_INT, [_P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _INT, _P, _P]),
     "tb200_ragged_gemm_dgrad": (_INT, [_P, _P, _P, _P, _I32, _I64, _I32, _I32, _INT, _P, _P]),
     "tb200_ragged_wgrad_workspace_bytes": (_I64, [_I32, _I64, _I32, _I32]),
+    "tb200_ragged_wgrad_workspace_of": (_I64, [_I32, _I64, _I32, _I32, _I32]),
     "tb200_ragged_gemm_wgrad": (_INT, [_P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _INT, _P, _P]),
     "tb200_token_project_fwd": (
         _INT, [_P, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _P, _I64, _I32, _F, _F, _P, _P],

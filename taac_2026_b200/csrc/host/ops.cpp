@@ -757,7 +757,7 @@ PyObject* py_ragged_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t
     const auto opt = x.options().requires_grad(false);
     Tensor dx = at::empty(x.sizes(), opt), dw = at::empty(w.sizes(), opt), db;
     if (bias) db = at::empty({r.experts, r.n}, opt.dtype(at::kFloat));
-    Tensor work = at::empty({std::max<int64_t>(tb200_ragged_wgrad_workspace_bytes(e, r.rows, n, k) / 4, 1)}, opt.dtype(at::kFloat));
+    Tensor work = at::empty({std::max<int64_t>(tb200_ragged_wgrad_workspace_of(e, r.rows, n, k, 1) / 4, 1)}, opt.dtype(at::kFloat));
     const auto* offsets = off.data_ptr<int32_t>();
     int code = tb200_ragged_gemm_dgrad(ptr(dy), ptr(w), offsets, ptr(dx), e, r.rows, n, k, r.type, word, stream_of(x));
     if (code == TB200_OK)

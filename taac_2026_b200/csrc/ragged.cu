@@ -999,10 +999,16 @@ extern "C" int tb200_ragged_gemm_dgrad(const void* dy, const void* w, const int3
     return dtype == TB200_BF16 ? rows_of<__nv_bfloat16>(dy, w, g, N, K, true, st) : rows_of<__half>(dy, w, g, N, K, true, st);
 }
 
-extern "C" int64_t tb200_ragged_wgrad_workspace_bytes(int32_t experts, int64_t T, int32_t N, int32_t K) {
+// Partial tiles where dw is wanted, else the table of the kernel that adds the bias gradient's rows alone
+extern "C" int64_t tb200_ragged_wgrad_workspace_of(int32_t experts, int64_t T, int32_t N, int32_t K, int32_t weights) {
     using namespace tb200;
     if (checked(experts, T, N, K, TB200_BF16) != TB200_OK || experts == 0 || !device_info().valid) return 0;
-    return 4 * (share_floats(experts, T, N, K) + (bias_shape(T, N).chunks + experts) * N);
+    return 4 * (weights ? share_floats(experts, T, N, K) : (bias_shape(T, N).chunks + experts) * N);
+}
+
+extern "C" int64_t tb200_ragged_wgrad_workspace_bytes(int32_t experts, int64_t T, int32_t N, int32_t K) {
+    const int64_t with = tb200_ragged_wgrad_workspace_of(experts, T, N, K, 1), without = tb200_ragged_wgrad_workspace_of(experts, T, N, K, 0);
+    return with > without ? with : without;
 }
 
 extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int32_t* offsets, void* dw, float* db, float* workspace, int32_t experts,
@@ -1030,17 +1036,16 @@ extern "C" int tb200_ragged_gemm_wgrad(const void* x, const void* dy, const int3
     g.T = T;
     g.cols = K;
     g.n = N;
-    const int64_t shared = share_floats(experts, T, N, K);
-    if (shared > 0) {
-        g.pieces = reinterpret_cast<int4*>(workspace);
-        g.db_partial = workspace + pairs_here() * 8;
-        g.partial = g.db_partial + pairs_here() * 2 * kTile;
-    }
     if (dw != nullptr) {
+        if (share_floats(experts, T, N, K) > 0) {
+            g.pieces = reinterpret_cast<int4*>(workspace);
+            g.db_partial = workspace + pairs_here() * 8;
+            g.partial = g.db_partial + pairs_here() * 2 * kTile;
+        }
         g.db = db;
         return dtype == TB200_BF16 ? weights_of<__nv_bfloat16>(x, dy, g, st) : weights_of<__half>(x, dy, g, st);
     }
-    float* part = workspace + shared;
+    float* part = workspace;
     const BiasShape b = bias_shape(T, N);
     const dim3 grid(static_cast<unsigned>(b.chunks), b.columns), block(b.tx, 256 / b.tx);
     const size_t rows = (static_cast<size_t>(experts) + 1) * 4, smem = static_cast<size_t>(256 / b.tx - 1) * b.tx * 8 * 4 + rows;

@@ -1880,7 +1880,8 @@ def ragged_linear_backward(x: torch.Tensor, weight: torch.Tensor, offsets: torch
             kept = None if not need_weight else _aligned(x.detach()) if scales is None else restore_activation(x, scales, dy.dtype)
             dw = torch.empty(experts, n, k, dtype=dy.dtype, device=dev) if need_weight else None
             db = torch.empty(experts, n, dtype=torch.float32, device=dev) if bias else None
-            work = torch.empty(max(int(lib.tb200_ragged_wgrad_workspace_bytes(experts, rows, n, k)) // 4, 1), dtype=torch.float32, device=dev)
+            size = int(lib.tb200_ragged_wgrad_workspace_of(experts, rows, n, k, int(need_weight)))
+            work = torch.empty(max(size // 4, 1), dtype=torch.float32, device=dev)
             with _timed("ragged_linear_wgrad", experts=experts, m=n, n=k, k=rows):
                 code = lib.tb200_ragged_gemm_wgrad(_ptr(kept), _ptr(dy), _ptr(off), _ptr(dw), _ptr(db), _ptr(work), experts, rows, n, k, dt,
                                                    _ptr(status), _stream_ptr())
