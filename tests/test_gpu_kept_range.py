@@ -93,3 +93,24 @@ def test_weight_gradient_of_a_kept_input_at_the_end_of_the_range(dtype):
     kept[3], kept[11] = 0, 0                              # rows that the gradient does not look at: any value is right
     values = ops.restore_activation(*ops.checkpoint_activation(kept), dtype)
     assert torch.equal(weight.grad, ops.ragged_linear_backward(values, w, off, dy)[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_than_two_dimensions(dtype):
+    """[4, 10, 512] and a strided view of it: the bits of the matrix of its rows, in its shape."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(4, 10, 512, generator=g, device="cuda").to(dtype)
+    pad = torch.zeros(4, 11, 520, device="cuda", dtype=dtype)
+    pad[:, :10, 3:515] = x
+    bits = lambda ts: [t.contiguous().view(torch.uint8).flatten() for t in ts]  # noqa: E731
+    for y in (x, pad[:, :10, 3:515]):
+        q, s = ops.checkpoint_activation(y)
+        assert q.shape == (4, 10, 512) and s.shape == (4, 10, 4)
+        assert all(torch.equal(a, b) for a, b in zip(bits((q, s)), bits(ops.checkpoint_activation(x.view(40, 512)))))
+        assert torch.equal(ops.restore_activation(q, s, dtype).view(40, 512), ops.restore_activation(q.view(40, 512), s.view(40, 4), dtype))
+        h, q, s = ops.silu_gate_checkpoint(y)
+        assert h.shape == (4, 10, 256) and q.shape == (4, 10, 512) and s.shape == (4, 10, 4)
+        assert all(torch.equal(a, b) for a, b in zip(bits((h, q, s)), bits(ops.silu_gate_checkpoint(x.view(40, 512)))))
+        dup, again = ops.silu_gate_backward(q, s, h)
+        assert dup.shape == (4, 10, 512) and again.shape == (4, 10, 256)
+        assert all(torch.equal(a, b) for a, b in zip(bits((dup, again)), bits(ops.silu_gate_backward(q.view(40, 512), s.view(40, 4), h.view(40, 256)))))
