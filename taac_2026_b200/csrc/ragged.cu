@@ -895,7 +895,11 @@ constexpr int64_t kShareRows = 2 * kSnap * kBlock;
 // bias gradient, in us: 16 experts of 128 rows, 512 -> 2048, 15.8 / 20.4, of 512 29.1 / 30.0, of 1024 49.6 / 46.5; 256 of 128 rows, 512 -> 512,
 // 48 / 61; one of 1000, 512 -> 512, 10.2 / 21.0, of 8000 17.5 / 27.0, of 60000 75.6 / 54.2; 20 of 1500, 256 -> 256, 17.2 / 25.3; 2 of 3000,
 // 512 -> 2048, 24.9 / 33.1; 4 of 10000, 1024 -> 1024, 132.8 / 108.8; one of 100000, 128 -> 128, 102.9 / 58.5.
+// A CTA of the other kernel may get the whole chain of blocks of an expert that has all the rows (0.54 us a block), and its waits end after
+// two seconds: from kMostChained rows on, 0.57 s, the pairs, which share such a tile, serve the call whatever the times are.
+constexpr int64_t kMostChained = int64_t(1) << 26;
 bool few_weights(int32_t experts, int64_t T, int32_t N, int32_t K) {
+    if (T > kMostChained) return false;
     const auto tiles = [&](int tile) { return static_cast<int64_t>(experts) * ((N + tile - 1) / tile) * ((K + tile - 1) / tile); };
     const int64_t blocks = (T / experts + kBlock - 1) / kBlock, small = tiles(128), large = tiles(kTile), pairs = pairs_here(), here = 4 * pairs;
     const int64_t split = weights_split(small, blocks, here), part = (blocks + split - 1) / split;

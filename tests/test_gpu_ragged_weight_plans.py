@@ -32,6 +32,8 @@ def _pairs():
 def _few(experts, rows, n, k):
     """0: pairs of CTAs; else how many CTAs share a 128 x 128 tile.  Expected times, in hundredths of a microsecond."""
     pairs, here = _pairs(), 4 * _pairs()
+    if rows > 1 << 26:
+        return 0
     blocks = _up(rows // experts, 64)
     small, large = (experts * _up(n, t) * _up(k, t) for t in (128, 256))
     split = next((s for s in (8, 4, 2) if s * small <= here and blocks >= 4 * s and blocks >= 12), 1)
@@ -105,6 +107,27 @@ def test_the_rule_is_the_one_stated_here():
                 assert (lib.tb200_ragged_wgrad_workspace_of(experts, rows, n, k, 1) > 0) == pairs, (experts, rows, n, k)
                 seen.add(pairs)
     assert seen == {True, False}
+
+
+def test_the_longest_chain_is_shared():
+    """300 experts, one of them with 270 million rows: one CTA's chain of 4.2 million blocks would outlast its bounded waits (2.2 s), so
+    pairs share it.  The values are 1, 0 and -1, every 2^20th row: fp32 sums them without rounding."""
+    experts, long, n, k = 300, 270_000_000, 8, 8
+    rows = long + experts - 1
+    assert _few(experts, rows, n, k) == 0
+    x, dy = (torch.zeros(rows, c, device="cuda", dtype=torch.bfloat16) for c in (k, n))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for t in (x, dy):
+        some = t[::1 << 20]
+        some.copy_(torch.randint(-1, 2, some.shape, generator=g, device="cuda"))
+        t[long:] = torch.randint(-1, 2, t[long:].shape, generator=g, device="cuda").bfloat16()
+    off = torch.cat([torch.zeros(1, dtype=torch.int32), torch.arange(long, rows + 1, dtype=torch.int32)]).cuda()
+    w = torch.zeros(experts, n, k, device="cuda", dtype=torch.bfloat16)
+    _dx, dw, db = ops.ragged_linear_backward(x, w, off, dy, bias=True, need_x=False, check=True)
+    xs, ds = x[:long:1 << 20].double(), dy[:long:1 << 20].double()
+    assert torch.equal(dw[0].double(), ds.T @ xs) and torch.equal(db[0].double(), ds.sum(0))
+    want = dy[long:].double()[:, :, None] * x[long:].double()[:, None]
+    assert torch.equal(dw[1:].double(), want) and torch.equal(db[1:].double(), dy[long:].double())
 
 
 def test_two_pair_plans_at_once():
