@@ -885,17 +885,21 @@ int rows_of(const void* x, const void* w, RaggedArgs g, int32_t N, int32_t K, bo
     return launch_pairs<T, kRows, false, false>(ta, tb, to, g, pairs, st);
 }
 
-// rows from which on a tile can be shared by pairs: with fewer, no expert has 2 kSnap blocks
+// rows from which on partial tiles are provided for: with fewer a tile has 2 kSnap blocks at most, which a cut would not shorten
 constexpr int64_t kShareRows = 2 * kSnap * kBlock;
 
 // Whether the weight gradients go to the kernel of 128 x 128 tiles: where it is expected to end first, by times (in hundredths of a us) that
-// come close to those measured over all sizes.  There a CTA takes 0.65 us a block of 64 rows and five blocks' time a tile at least, two CTAs
-// share an SM, and clusters add 3 us.  Here a pair takes 0.53 us a block and seven blocks' time at least, with whole tiles or in equal
-// shares; the partial tiles of those and their sum, of as many as share a tile, come on top.  Measured, 128 x 128 / pairs, with a
-// bias gradient, in us: 16 experts of 128 rows, 512 -> 2048, 15.8 / 20.4, of 512 29.1 / 30.0, of 1024 49.6 / 46.5; 256 of 128 rows, 512 -> 512,
+// come close to those measured where the experts have similar numbers of rows: the host sees T / experts only.  There a CTA takes 0.65 us a
+// block of 64 rows while two busy ones share its SM (0.3 to 0.55 alone) and five blocks' time a tile at least, and clusters add 3 us.  Here a
+// pair takes 0.53 us a block and seven blocks' time at least, with whole tiles or in equal shares; the partial tiles of those and their
+// sum, of as many as share a tile, come on top.  Measured, 128 x 128 / pairs, with a bias gradient, in us: 16 experts of 128 rows, 512 -> 2048, 15.8 / 20.4, of 512 29.1 / 30.0, of 1024 49.6 / 46.5; 256 of 128 rows, 512 -> 512,
 // 48 / 61; one of 1000, 512 -> 512, 10.2 / 21.0, of 8000 17.5 / 27.0, of 60000 75.6 / 54.2; 20 of 1500, 256 -> 256, 17.2 / 25.3; 2 of 3000,
 // 512 -> 2048, 24.9 / 33.1; 4 of 10000, 1024 -> 1024, 132.8 / 108.8; one of 100000, 128 -> 128, 102.9 / 58.5.
-// A CTA of the other kernel may get the whole chain of blocks of an expert that has all the rows (0.54 us a block), and its waits end after
+// Where one expert has most of the rows this rule is wrong: the mean says single CTAs, and its tiles' chains, shared by nobody, decide the
+// time.  One of 32768 rows beside 16 of 128, 512 -> 512: 290 us, 25 with even experts; of 16384 beside 16 of 64: 137 and 15; of 131072
+// beside 32 of 512, 128 -> 128: 131 and 19.
+//
+// A CTA of the 128 x 128 kernel may get the whole chain of blocks of an expert that has all the rows (0.54 us a block), and its waits end after
 // two seconds: from kMostChained rows on, 0.57 s, the pairs, which share such a tile, serve the call whatever the times are.
 constexpr int64_t kMostChained = int64_t(1) << 26;
 bool few_weights(int32_t experts, int64_t T, int32_t N, int32_t K) {
