@@ -298,8 +298,8 @@ add_norm_bwd_kernel(const BwdArgs<T> a) {
             }
         }
         const float2 sums = row_sum<G <= 1 ? 0 : G>(make_float2(ss.x + ss.y, gt.x + gt.y), slots[parity], warp0, warps);
-        // without a row (half of a last warp) nothing is added to dw: 0 x infinity would be, where eps is 0
-        const float s = row < a.rows ? rsqrtf(sums.x * inv_cols + a.eps) : 0.f;
+        // without a row (half of a last warp) s is 1, so that nothing is added to dw: with eps = 0 it would be 0 x infinity
+        const float s = rsqrtf(sums.x * inv_cols + (G == 16 && row >= a.rows ? 1.0f : a.eps));
         const float2 s2 = make_float2(s, s), k2 = make_float2(-(s * s) * (sums.y * inv_cols), -(s * s) * (sums.y * inv_cols));
 #pragma unroll
         for (int j = 0; j < PPL; ++j) {

@@ -283,7 +283,6 @@ gate_bwd_kernel(const void* __restrict__ from, const float* __restrict__ scales,
             sg[u].values(g);
             const int64_t ig = (in[u] + to_gate) * 8;
             if (MODE == 0) {
-                if (huge_scale(sg[u].s)) finite(g);
                 store_held(dup + ig, g);
                 continue;
             }
