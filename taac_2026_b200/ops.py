@@ -438,8 +438,8 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     """``total = x + residual`` and ``normed = rms_norm(total, weight, eps)`` in one pass: the residual stream and the input
     of a block's next layer (`x + attention(...)`, `ffn_norm`: experiments/onetrans/model.py:106-107).
 
-    The statistics come from the sum in fp32, before it is rounded.  Differentiable: both results may have upstream
-    gradients.  The width is a multiple of 8, at most 16384."""
+    The statistics come from the sum in fp32, before it is rounded; ``weight`` is used in x's dtype, as in ``rms_norm``.
+    Differentiable: both results may have upstream gradients.  The width is a multiple of 8, at most 16384."""
     _require_backend_name("add_rms_norm", backend)
     if residual is None:
         raise ValueError("add_rms_norm needs a residual; rms_norm serves a single input")
@@ -478,7 +478,8 @@ def add_rms_norm_quant(x: torch.Tensor, residual: torch.Tensor | None, weight: t
 def add_rms_norm_backward(total: torch.Tensor, weight: torch.Tensor, grad_normed: torch.Tensor, grad_total: torch.Tensor | None = None,
                           eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
     """(grad, dweight) of ``add_rms_norm``: ``grad`` is the gradient of x and of residual alike, from the upstream gradients of
-    ``normed`` and (None: zero) of ``total``.  Statistics recomputed from ``total`` in fp32; sums in a fixed order."""
+    ``normed`` and (None: zero) of ``total``.  Statistics recomputed from ``total`` in fp32; the weight's gradient is summed over the
+    rows in fp32, in a fixed order, and has total's dtype."""
     if _TIMING is None:
         fast = _host.add_rms_norm_backward(total, weight, grad_normed, grad_total, eps)
         if fast is not None:
